@@ -1,0 +1,560 @@
+"""The engine's language-model operators as cases that can be timed and compared: a key/value cache held in Q4_0 or
+Q8_0 (written, read back), attention over it, and the matrix product that ends in an activation and a residual add.
+
+With `own` false an operator is computed in its plain form, elementary torch operations in 32 bits; with `own` true by
+the engine, through the C ABI's Python binding. Sizes are the engine's: the ViT's width 1024 in 16 heads, its MLP of
+4736 and the 5184 tokens of a 1008 px image, the memory bank's 28 736 tokens of width 256, the text encoder's 16 heads
+of 64; and generic ones: 32 query heads on 8 key/value heads of 128.
+"""
+import math
+import os
+import random
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda"
+Q4_0, Q8_0 = 2, 8  # ggml type ids
+GGML_TYPES = {"f32": 0, "f16": 1, "q4_0": Q4_0, "q4_1": 3, "q8_0": Q8_0}
+BYTES_PER_WEIGHT = {"q4_0": 18 / 32, "q4_1": 20 / 32, "q8_0": 34 / 32, "f16": 2.0, "f32": 4.0}
+FLOAT = {"f32": torch.float32, "f16": torch.float16}
+
+# (N, K) of the engine's linears: the ViT's proj, fc1 and fc2; Hiera's; the memory attention's
+LINEARS = [(1024, 1024), (4736, 1024), (1024, 4736), (672, 224), (896, 3584), (1152, 384), (384, 1536), (768, 256),
+           (256, 64), (2048, 256), (256, 2048)]
+ACTS = ["none", "relu", "gelu_erf", "gelu_tanh", "silu"]
+
+
+def listed():
+    return [
+        # one new token of each of 8 short texts, in the text encoder's 16 heads of 64: launches and latency
+        {"name": "cache_token_q4_0", "kind": "cache", "type": "q4_0", "io": "f32", "n": 8, "heads": 16, "D": 64,
+         "page": 32, "order": "scatter", "fused": True},
+        # the tokens of one 1008 px image at once, starting inside a page
+        {"name": "cache_image_q4_0", "kind": "cache", "type": "q4_0", "io": "f32", "n": 5184, "heads": 16, "D": 64,
+         "page": 64, "order": "run", "fused": True},
+        # a long document's keys and values, fp16
+        {"name": "cache_long_q4_0", "kind": "cache", "type": "q4_0", "io": "f16", "n": 65536, "heads": 8, "D": 128,
+         "page": 64, "order": "run", "fused": False},
+        # a full memory bank: 7 frames of 64 x 64 tokens and 64 object-pointer tokens of one head of 256
+        {"name": "cache_bank_q8_0", "kind": "cache", "type": "q8_0", "io": "f16", "n": 28736, "heads": 1, "D": 256,
+         "page": 256, "order": "run", "fused": False},
+        # the next token of one short text: launches and latency
+        {"name": "attn_token_q4_0", "kind": "attn", "type": "q4_0", "io": "f32", "seqs": 1, "nq": 1, "kv": 77,
+         "nh": 16, "heads": 16, "D": 64, "page": 32, "mask": "causal", "mix": 1},
+        # the next token of 64 sequences of mixed lengths, grouped heads
+        {"name": "attn_batch_q4_0", "kind": "attn", "type": "q4_0", "io": "f16", "seqs": 64, "nq": 1, "kv": 4096,
+         "nh": 32, "heads": 8, "D": 128, "page": 64, "mask": "causal", "mix": 2},
+        # the next token after a long document
+        {"name": "attn_long_q4_0", "kind": "attn", "type": "q4_0", "io": "f16", "seqs": 1, "nq": 1, "kv": 131072,
+         "nh": 32, "heads": 8, "D": 128, "page": 128, "mask": "causal", "mix": 3},
+        # five drafted tokens a sequence under a tree's mask, with rows that see nothing, in f32
+        {"name": "attn_draft_q8_0", "kind": "attn", "type": "q8_0", "io": "f32", "seqs": 7, "nq": 5, "kv": 1733,
+         "nh": 16, "heads": 4, "D": 128, "page": 64, "mask": "dense", "mix": 4},
+        # a first pass over four prompts of ragged lengths, causal
+        {"name": "attn_prompt_q4_0", "kind": "attn", "type": "q4_0", "io": "f16", "seqs": 4, "nq": 2048, "kv": 2592,
+         "nh": 16, "heads": 16, "D": 64, "page": 64, "mask": "causal", "mix": 5},
+        # a frame's 64 x 64 tokens against a full memory bank held in 8 bits
+        {"name": "attn_bank_q8_0", "kind": "attn", "type": "q8_0", "io": "f16", "seqs": 1, "nq": 4096, "kv": 28736,
+         "nh": 1, "heads": 1, "D": 256, "page": 256, "mask": "none", "mix": 6},
+        # a few decoder tokens through an output projection, added to the residual stream
+        {"name": "product_tokens_q4_0", "kind": "product", "type": "q4_0", "M": 7, "N": 1024, "K": 1024, "bias": True,
+         "act": "none", "residual": True},
+        # the ViT's fc1 and GELU over an image's tokens
+        {"name": "product_fc1_q8_0", "kind": "product", "type": "q8_0", "M": 5184, "N": 4736, "K": 1024, "bias": True,
+         "act": "gelu_erf", "residual": False},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case of the listed ones' ranges."""
+    kind = rng.choice(["cache", "attn", "attn", "product"])
+    type_ = rng.choice(["q4_0", "q4_0", "q8_0"])
+    D = rng.choice([32, 64, 64, 96, 128, 128, 256])
+    page = rng.choice([32, 64, 128, 256])
+    if kind == "cache":
+        heads = _log_int(rng, 1, 16)
+        return {"kind": kind, "type": type_, "io": rng.choice(["f16", "f32"]), "n": _log_int(rng, 1, 2 ** 25 // (heads * D)),
+                "heads": heads, "D": D, "page": page, "order": rng.choice(["run", "run", "scatter"]),
+                "fused": rng.random() < 0.5}
+    if kind == "attn":
+        heads, group = rng.choice([1, 2, 3, 4, 8]), rng.choice([1, 1, 2, 4, 5, 8])
+        form = rng.choice(["token", "token", "few", "prompt"])
+        seqs = _log_int(rng, 1, 48) if form != "prompt" else rng.randint(1, 3)
+        nq = 1 if form == "token" else rng.randint(2, 9) if form == "few" else _log_int(rng, 16, 1500)
+        kv = _log_int(rng, 1, 2 ** 24 // (seqs * heads * D))
+        kv = min(kv, 5000) if form == "prompt" else min(kv, 100000)
+        return {"kind": kind, "type": type_, "io": rng.choice(["f16", "f16", "f32"]), "seqs": seqs, "nq": nq,
+                "kv": max(kv, nq), "nh": heads * group, "heads": heads, "D": D, "page": page,
+                "mask": rng.choice(["causal", "causal", "none", "dense"]), "mix": rng.randrange(1 << 20)}
+    if rng.random() < 0.7:
+        N, K = rng.choice(LINEARS)
+    else:
+        N, K = _log_int(rng, 33, 4736), 32 * _log_int(rng, 2, 148)
+    return {"kind": kind, "type": rng.choice(["q4_0", "q4_0", "q8_0", "q8_0", "f16", "q4_1", "f32"]),
+            "M": _log_int(rng, 1, min(5184, 5184 * 4736 * 1024 // (N * K))), "N": N, "K": K, "bias": rng.random() < 0.8, "act": rng.choice(ACTS),
+            "residual": rng.random() < 0.5}
+
+
+# ---- inputs --------------------------------------------------------------------
+def _randn(gen, *shape):
+    return torch.randn(*shape, generator=gen, device=DEV, dtype=torch.float32)
+
+
+def _first_of_largest(b):
+    """The first value of largest magnitude of each block (last axis)."""
+    a = b.abs()
+    at = torch.where(a == a.amax(-1, keepdim=True), torch.arange(b.shape[-1], device=b.device), b.shape[-1])
+    return torch.gather(b, -1, at.amin(-1, keepdim=True))[..., 0]
+
+
+def _quantize(type_, x):
+    """Rows of f32 to block codes and fp16 scales as ggml converts them: codes uint8 0..15 (q4_0) or int8 (q8_0), of
+    x's shape, scales [..., D / 32]."""
+    b = x.reshape(*x.shape[:-1], -1, 32)
+    if type_ == "q4_0":
+        d = _first_of_largest(b) / -8
+        inv = torch.where(d != 0, torch.ones_like(d) / d, torch.zeros_like(d))
+        q = torch.clamp(torch.floor(b * inv[..., None] + 8.5), max=15).to(torch.uint8)
+    else:
+        amax = b.abs().amax(-1)
+        top = torch.full_like(amax, 127)  # tensors: divided as IEEE does, not by a reciprocal
+        d = amax / top
+        inv = torch.where(amax > 0, top / amax, torch.zeros_like(amax))
+        q = torch.round(b * inv[..., None]).to(torch.int8)
+    return q.reshape(x.shape), d.half()
+
+
+def _values(type_, q, d):
+    """The f32 values of codes and scales."""
+    c = q.float() - 8 if type_ == "q4_0" else q.float()
+    return (c.reshape(*d.shape, 32) * d.float()[..., None]).reshape(q.shape)
+
+
+def _lengths(case):
+    """(queries, keys) of each sequence, by the case alone: one of full length, the others spread below it."""
+    r, out = random.Random(case["mix"]), []
+    for i in range(case["seqs"]):
+        kv = case["kv"] if i == 0 else max(1, int(case["kv"] * r.random()))
+        nq = case["nq"] if i == 0 or case["nq"] < 16 else max(1, int(case["nq"] * r.random()))
+        out.append((nq, kv))
+    return out
+
+
+def _attn_inputs(case, seed):
+    """Codes and scales of K and V by page slot, the page table, and q."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    lens, page, H, D = _lengths(case), case["page"], case["heads"], case["D"]
+    need = [-(-kv // page) for _, kv in lens]
+    n_pages = sum(need) + 1
+    perm = torch.randperm(n_pages, generator=gen, device=DEV).to(torch.int32)
+    table = torch.zeros(len(lens), max(need), dtype=torch.int32, device=DEV)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = perm[at:at + n]
+        at += n
+    shape = (n_pages * page, H, D)
+    k = _quantize(case["type"], _randn(gen, *shape))
+    # channels of unlike size, as values have them
+    v = _quantize(case["type"], _randn(gen, *shape) * torch.exp(0.5 * _randn(gen, D)) + 0.1)
+    n_tokens = sum(nq for nq, _ in lens)
+    q = _randn(gen, n_tokens, case["nh"], D).to(FLOAT[case["io"]])
+    mask = None
+    if case["mask"] == "dense":
+        # open, but for the drafted keys that are not a token's ancestors; now and then a row that sees nothing
+        L = max(kv for _, kv in lens)
+        mask = torch.where(torch.rand(n_tokens, L, generator=gen, device=DEV) < 0.1, float("-inf"), 0.0)
+        mask += 0.5 * _randn(gen, n_tokens, L)
+        mask[torch.rand(n_tokens, generator=gen, device=DEV) < 0.1] = float("-inf")
+        mask = mask.half()
+    return {"k": k, "v": v, "table": table, "q": q, "mask": mask, "lens": lens, "n_pages": n_pages}
+
+
+def _cache_inputs(case, seed):
+    """K and V rows [n][heads][D] (views of a fused projection's rows, or tensors of their own) and their slots."""
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    n, H, D, page = case["n"], case["heads"], case["D"], case["page"]
+    if case["fused"]:
+        rows = _randn(gen, n, 3 * H * D).to(FLOAT[case["io"]])
+        k, v = rows[:, H * D:2 * H * D].view(n, H, D), rows[:, 2 * H * D:].view(n, H, D)
+    else:
+        k, v = (_randn(gen, n, H, D).to(FLOAT[case["io"]]) for _ in range(2))
+    first = page // 2 + 3  # a sequence that goes on inside a page
+    n_pages = -(-(n + first) // page) + 1
+    if case["order"] == "run":
+        pages = torch.randperm(n_pages, generator=gen, device=DEV)
+        j = torch.arange(first, first + n, device=DEV)
+        slots = pages[j // page] * page + j % page
+    else:
+        slots = torch.randperm(n_pages * page, generator=gen, device=DEV)[:n]
+    return k, v, slots.to(torch.int32), n_pages
+
+
+def _weight_codes(type_, W):
+    """Block codes of weights as the reference quantizers choose them: (codes, fp16 scales, fp16 minima or None)."""
+    b = W.reshape(W.shape[0], -1, 32)
+    if type_ == "q4_0":
+        q, d = _quantize("q4_0", W)
+        return q.reshape(b.shape), d, None
+    if type_ == "q8_0":
+        d = b.abs().amax(-1) / 127
+        inv = torch.where(d > 0, torch.ones_like(d) / d, torch.zeros_like(d))
+        return torch.round(b * inv[..., None]).to(torch.int8), d.half(), None
+    lo, hi = b.amin(-1), b.amax(-1)
+    d = (hi - lo) / 15
+    inv = torch.where(d > 0, torch.ones_like(d) / d, torch.zeros_like(d))
+    return torch.clamp(torch.floor((b - lo[..., None]) * inv[..., None] + 0.5), max=15).to(torch.uint8), d.half(), lo.half()
+
+
+def _ggml_bytes(type_, W):
+    if type_ == "f32":
+        return W.cpu().numpy()
+    if type_ == "f16":
+        return W.half().cpu().numpy()
+    q, d, m = _weight_codes(type_, W)
+    parts = [x[..., None].contiguous().view(torch.uint8) for x in (d, m) if x is not None]
+    parts.append(q.view(torch.uint8) if type_ == "q8_0" else q[..., :16] | (q[..., 16:] << 4))
+    return torch.cat(parts, -1).reshape(W.shape[0], -1).contiguous().cpu().numpy()
+
+
+def _product_inputs(case, seed):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    X = _randn(gen, case["M"], case["K"])
+    W = _randn(gen, case["N"], case["K"]) * 0.02
+    bias = _randn(gen, case["N"]) * 0.1 if case["bias"] else None
+    R = _randn(gen, case["M"], case["N"]) if case["residual"] else None
+    return X, W, bias, R
+
+
+# ---- the engine's cache, as its header documents the bytes -----------------------
+def _words(codes, bits):
+    """codes [..., 8] of one word each to bytes [..., bits]: 8-bit words in order; of 4-bit words, code j is the nibble
+    (j >> 1) + 4 * (j & 1)."""
+    if bits == 8:
+        return codes.view(torch.uint8)
+    c = codes[..., [0, 2, 4, 6, 1, 3, 5, 7]]
+    return c[..., 0::2] | (c[..., 1::2] << 4)
+
+
+def _pieces(words):
+    """[..., w, lane, bytes] to the byte string of a chunk: 16 bytes of each lane, then the next 16."""
+    lead, (W, _, B) = words.shape[:-3], words.shape[-3:]
+    per = 16 // B
+    out = [words[..., w:w + per, :, :].transpose(-3, -2).reshape(*lead, -1) for w in range(0, W, per)]
+    return torch.cat(out, -1)
+
+
+def _native(type_, k, v, page):
+    """The cache's bytes [pages, heads, page / 32, chunk] of codes and scales by slot."""
+    (kq, kd), (vq, vd) = k, v
+    bits = 4 if type_ == "q4_0" else 8
+    S, H, D = kq.shape
+    NB, G = D // 32, S // 32
+    # keys 8a + 4t + i and channels 32b + 8g + j: word (t, b) of lane (g, a, i) holds the eight j
+    kw = _words(kq.reshape(G, 4, 2, 4, H, NB, 4, 8), bits).permute(0, 4, 2, 5, 6, 1, 3, 7)
+    kw = _pieces(kw.reshape(G, H, 2 * NB, 64, bits))
+    # channels 16w + m and keys 8g + j: word w of lane (g, m) holds the eight j
+    vw = _words(vq.reshape(G, 4, 8, H, 2 * NB, 16).permute(0, 3, 4, 1, 5, 2).contiguous(), bits)
+    vw = _pieces(vw.reshape(G, H, 2 * NB, 64, bits))
+    ks, vs = (d.reshape(G, 32, H, NB).permute(0, 2, 3, 1).contiguous().view(torch.uint8).reshape(G, H, -1) for d in (kd, vd))
+    chunk = torch.cat([kw, ks, vw, vs], -1)
+    return chunk.reshape(-1, page // 32, H, chunk.shape[-1]).transpose(1, 2).contiguous()
+
+
+# ---- what a program holds before the call ----------------------------------------
+_held = {}
+
+
+def _engine():
+    """The engine's binding and one context."""
+    if "ctx" not in _held:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sam3.cpp_amd"))
+        import s3e
+        _held["s3e"], _held["ctx"] = s3e, s3e.Context(0)
+    return _held["s3e"], _held["ctx"]
+
+
+def _buf(t):
+    return None if t is None else _held["s3e"].DeviceView(t.data_ptr(), t.numel() * t.element_size())
+
+
+def _prepare_cache(case, seed):
+    k, v, slots, n_pages = _cache_inputs(case, seed)
+    H, D, n = case["heads"], case["D"], case["n"]
+    bytes_ = n_pages * case["page"] * H * D * (9 if case["type"] == "q4_0" else 17) // 8
+    s = {"k": k, "v": v, "slots": slots, "data": torch.zeros(bytes_, dtype=torch.uint8, device=DEV)}
+    # the plain form's cache: codes and scales by slot
+    slots_all, half = n_pages * case["page"], 2 if case["type"] == "q4_0" else 1
+    s["codes"] = [torch.zeros(slots_all, H, D // half, dtype=torch.uint8 if half == 2 else torch.int8, device=DEV) for _ in "kv"]
+    s["scales"] = [torch.zeros(slots_all, H, D // 32, dtype=torch.float16, device=DEV) for _ in "kv"]
+    s["out"] = [torch.empty(n, H, D, dtype=FLOAT[case["io"]], device=DEV) for _ in "kv"]
+    if own:
+        s3e, ctx = _engine()
+        s["cache"] = s3e.KVCache(GGML_TYPES[case["type"]], H, D, case["page"], n_pages, _buf(s["data"]))
+    return s
+
+
+def _prepare_attn(case, seed):
+    s = _attn_inputs(case, seed)
+    lens = s["lens"]
+    s["data"] = _native(case["type"], s["k"], s["v"], case["page"])
+    if case["type"] == "q4_0":  # the plain form's cache: two codes a byte
+        s["k"], s["v"] = (((q[..., 0::2] | (q[..., 1::2] << 4)), d) for q, d in (s["k"], s["v"]))
+    starts = [0]
+    for nq, _ in lens:
+        starts.append(starts[-1] + nq)
+    s["starts"] = torch.tensor(starts, dtype=torch.int32, device=DEV)
+    s["kv_len"] = torch.tensor([kv for _, kv in lens], dtype=torch.int32, device=DEV)
+    s["max_q"], s["max_kv"] = max(nq for nq, _ in lens), max(kv for _, kv in lens)
+    s["o"] = torch.empty(starts[-1], case["nh"], case["D"], dtype=FLOAT[case["io"]], device=DEV)
+    s["scale"] = 1 / math.sqrt(case["D"])
+    if own:
+        s3e, ctx = _engine()
+        s["cache"] = s3e.KVCache(GGML_TYPES[case["type"]], case["heads"], case["D"], case["page"], s["n_pages"], _buf(s["data"]))
+        s["batch"] = s3e.KVBatch(len(lens), starts[-1], s["max_q"], s["max_kv"], _buf(s["starts"]), _buf(s["kv_len"]),
+                                 _buf(s["table"]), s["table"].shape[1])
+        need = s3e.kv_attn_workspace(s["cache"], s["batch"], case["nh"], GGML_TYPES[case["io"]])
+        s["ws"] = torch.empty(max(need, 16), dtype=torch.uint8, device=DEV)
+    return s
+
+
+def _prepare_product(case, seed):
+    X, W, bias, R = _product_inputs(case, seed)
+    s = {"X": X, "bias": bias, "R": R, "Y": torch.empty(case["M"], case["N"], device=DEV)}
+    if own:
+        s3e, ctx = _engine()
+        s["w"] = ctx.weight(GGML_TYPES[case["type"]], case["K"], case["N"], _ggml_bytes(case["type"], W))
+        s["ws"] = torch.empty(max(s3e.mul_mat_act_workspace(s["w"], case["M"]), 16), dtype=torch.uint8, device=DEV)
+        return s
+    # the plain form keeps the weights' values, and Q4_1's minima apart
+    s["minima"] = None
+    if case["type"] in ("f32", "f16"):
+        s["W"] = W if case["type"] == "f32" else W.half().float()
+    else:
+        q, d, m = _weight_codes(case["type"], W)
+        c = q.float() - 8 if case["type"] == "q4_0" else q.float()
+        s["W"], s["minima"] = (c * d.float()[..., None]).reshape(W.shape), None if m is None else m.float()
+    return s
+
+
+def prepare(case, seed):
+    s = {"cache": _prepare_cache, "attn": _prepare_attn, "product": _prepare_product}[case["kind"]](case, seed)
+    s["case"] = case
+    # the engine's stream is not torch's: what torch made must be there before the first call
+    torch.cuda.synchronize()
+    return s
+
+
+# ---- one call: the plain forms ----------------------------------------------------
+def _unpack(type_, q):
+    return torch.stack([q & 15, q >> 4], -1).flatten(-2) if type_ == "q4_0" else q
+
+
+def _plain_cache(s):
+    type_, at = s["case"]["type"], s["slots"].long()
+    out = []
+    for x, codes, scales in zip((s["k"], s["v"]), s["codes"], s["scales"]):
+        q, d = _quantize(type_, x.float())
+        codes[at] = (q[..., 0::2] | (q[..., 1::2] << 4)) if type_ == "q4_0" else q
+        scales[at] = d
+        out.append(_values(type_, _unpack(type_, codes[at]), scales[at]).to(x.dtype))
+    return out
+
+
+def _plain_attn(s):
+    case, q = s["case"], s["q"].float()
+    page, H, D, S, Q, L = case["page"], case["heads"], case["D"], case["seqs"], s["max_q"], s["max_kv"]
+    G = case["nh"] // H
+    j, i = torch.arange(L, device=DEV), torch.arange(Q, device=DEV)
+    slot = s["table"].long()[:, j // page] * page + j % page  # [S, L]
+    K, V = (_values(case["type"], _unpack(case["type"], codes[slot]), d[slot]) for codes, d in (s["k"], s["v"]))
+    nq, kv = s["starts"].diff().long(), s["kv_len"].long()
+    token = (s["starts"][:-1].long()[:, None] + i).clamp(max=q.shape[0] - 1)  # [S, Q]
+    qs = q[token].view(S, Q, H, G, D).permute(0, 2, 1, 3, 4).reshape(S, H, Q * G, D)
+    P = torch.matmul(qs, K.permute(0, 2, 3, 1)) * s["scale"]
+    P = P.view(S, H, Q, G, L)
+    see = (j < kv[:, None])[:, None, None, None]
+    if case["mask"] == "causal":
+        see = see & (j <= (kv - nq)[:, None, None] + i[:, None])[:, None, :, None]
+    if s["mask"] is not None:
+        P = P + s["mask"].float()[token][:, None, :, None]
+    P = torch.where(see, P, float("-inf"))
+    top = P.amax(-1, keepdim=True)
+    P = torch.exp(P - torch.where(top == float("-inf"), 0.0, top))
+    total = P.sum(-1, keepdim=True)
+    P = P / torch.where(total == 0, 1.0, total)
+    O = torch.matmul(P.view(S, H, Q * G, L), V.permute(0, 2, 1, 3)).view(S, H, Q, G, D).permute(0, 2, 1, 3, 4)
+    rows = (i < nq[:, None])
+    s["o"][token[rows]] = O[rows].reshape(-1, H * G, D).to(s["o"].dtype)
+    return s["o"]
+
+
+def _plain_product(s):
+    type_, X = s["case"]["type"], s["X"]
+    if type_ == "f16":
+        X = X.half().float()
+    elif type_ != "f32":
+        q, d = _quantize("q8_0", X)
+        amax = X.reshape(X.shape[0], -1, 32).abs().amax(-1)
+        X = _values("q8_0", q, d)
+    Y = torch.matmul(X, s["W"].T)
+    if s["minima"] is not None:  # Q8_1's block sums: of the scale before its rounding
+        sums = (amax / torch.full_like(amax, 127) * q.view(*d.shape, 32).float().sum(-1)).half().float()
+        Y = Y + torch.matmul(sums, s["minima"].T)
+    if s["bias"] is not None:
+        Y = Y + s["bias"]
+    act = s["case"]["act"]
+    if act == "relu":
+        Y = torch.where(Y > 0, Y, 0.0)
+    elif act == "gelu_erf":
+        Y = 0.5 * Y * (1 + torch.erf(Y * math.sqrt(0.5)))
+    elif act == "gelu_tanh":
+        Y = 0.5 * Y * (1 + torch.tanh(math.sqrt(2 / math.pi) * Y * (1 + 0.044715 * Y * Y)))
+    elif act == "silu":
+        Y = Y / (1 + torch.exp(-Y))
+    return Y if s["R"] is None else Y + s["R"]
+
+
+# ---- one call ----------------------------------------------------------------------
+def run(s):
+    kind, case = s["case"]["kind"], s["case"]
+    if not own:
+        return {"cache": _plain_cache, "attn": _plain_attn, "product": _plain_product}[kind](s)
+    s3e, ctx = _engine()
+    io = GGML_TYPES[case.get("io", "f32")]
+    if kind == "cache":
+        n, slots = case["n"], _buf(s["slots"])
+        k, v = s["k"], s["v"]
+        ctx.kv_write(s["cache"], io, _buf(k), k.stride()[:2], _buf(v), v.stride()[:2], slots, n)
+        ctx.kv_read(s["cache"], slots, n, io, *map(_buf, s["out"]))
+        return s["out"]
+    if kind == "attn":
+        q, mask = s["q"], s["mask"]
+        ctx.kv_attn(s["cache"], s["batch"], io, _buf(q), q.stride()[:2], case["nh"], s["scale"], _buf(s["o"]), _buf(s["ws"]),
+                    causal=case["mask"] == "causal", mask=_buf(mask), mask_ld=0 if mask is None else mask.stride(0))
+        return s["o"]
+    ctx.mul_mat_act(s["w"], _buf(s["X"]), case["M"], _buf(s["Y"]), _buf(s["ws"]), bias=_buf(s["bias"]), act=case["act"],
+                    residual=_buf(s["R"]))
+    return s["Y"]
+
+
+# ---- what the call cannot do without -------------------------------------------------
+def work(case):
+    if case["kind"] == "product":
+        M, N, K = case["M"], case["N"], case["K"]
+        bytes_ = N * K * BYTES_PER_WEIGHT[case["type"]] + 4 * M * (K + N) + (4 * N if case["bias"] else 0)
+        return {"bytes": bytes_ + (4 * M * N if case["residual"] else 0), "flops": 2 * M * N * K}
+    held, size = BYTES_PER_WEIGHT[case["type"]], 2 if case["io"] == "f16" else 4
+    if case["kind"] == "cache":
+        values = 2 * case["n"] * case["heads"] * case["D"]
+        # rows in and codes out; codes in and rows out; about ten operations a value
+        return {"bytes": 2 * values * (size + held) + 8 * case["n"], "flops": 10 * values}
+    rows = pairs = keys = masked = 0
+    for nq, kv in _lengths(case):
+        rows += nq
+        keys += kv
+        masked += nq * kv
+        # query i of nq sees keys up to kv - nq + i
+        pairs += sum(max(0, kv - nq + i + 1) for i in range(nq)) if case["mask"] == "causal" else nq * kv
+    bytes_ = 2 * keys * case["heads"] * case["D"] * held + 2 * rows * case["nh"] * case["D"] * size
+    return {"bytes": bytes_ + (2 * masked if case["mask"] == "dense" else 0), "flops": 4 * case["nh"] * case["D"] * pairs}
+
+
+# ---- the same in 64 bits --------------------------------------------------------------
+def _f32(x):
+    """A step of the definition that is rounded to fp32, in float64 again."""
+    return x.float().double()
+
+
+def _blocks_exact(type_, x):
+    """ggml's conversion of blocks [..., 32]: its fp32 steps (d, 1/d, the product, the sum) are part of what the codes
+    are. Codes from 0 around and fp16 scales as float64, and the scale before its rounding to fp16."""
+    x = x.double()
+    size, none = x.abs(), torch.zeros((), dtype=torch.float64, device=x.device)
+    if type_ == "q8_0":
+        top = size.max(-1, keepdim=True).values
+        d, inv = _f32(top / 127), torch.where(top > 0, _f32(127 / top), none)
+        q = torch.round(_f32(x * inv))  # half to even
+    else:
+        # the largest magnitude decides, of two such the earlier: rank by magnitude, then by place
+        lead = torch.argsort(size, dim=-1, descending=True, stable=True)[..., :1]
+        d = torch.gather(x, -1, lead) / -8
+        inv = torch.where(d != 0, _f32(1 / d), none)
+        q = torch.trunc(_f32(_f32(x * inv) + 8.5)).clamp(max=15) - 8
+    return q, d.half().double()[..., 0], d[..., 0]
+
+
+def _cache_exact(case, seed):
+    k, v, _, _ = _cache_inputs(case, seed)
+    out = []
+    for x in (k, v):
+        y = torch.empty_like(x, dtype=torch.float64, memory_format=torch.contiguous_format)
+        for a in range(0, x.shape[0], 4096):
+            part = x[a:a + 4096].contiguous()
+            q, d, _ = _blocks_exact(case["type"], part.view(*part.shape[:-1], -1, 32))
+            y[a:a + 4096] = (q * d[..., None]).reshape(part.shape)
+        out.append(y)
+    return out
+
+
+def _attn_exact(case, seed):
+    s = _attn_inputs(case, seed)
+    page, G, D = case["page"], case["nh"] // case["heads"], case["D"]
+    off, size = 8 if case["type"] == "q4_0" else 0, s["q"].shape[0]
+    O = torch.zeros(size, case["nh"], D, dtype=torch.float64, device=DEV)
+    at = 0
+    for i, (nq, kv) in enumerate(s["lens"]):
+        slot = (s["table"][i].long()[:, None] * page + torch.arange(page, device=DEV)).flatten()[:kv]
+        for h in range(case["heads"]):
+            k, v = ((q[slot, h].double() - off).view(kv, -1, 32) * d[slot, h].double()[..., None] for q, d in (s["k"], s["v"]))
+            k, v = k.view(kv, D), v.view(kv, D)
+            for a in range(0, nq, 1024):
+                b = min(nq, a + 1024)
+                rows = torch.arange(a, b, device=DEV)
+                hidden = torch.zeros(b - a, kv, dtype=torch.float64, device=DEV)
+                if case["mask"] == "causal":
+                    hidden[torch.arange(kv, device=DEV) > kv - nq + rows[:, None]] = float("-inf")
+                if s["mask"] is not None:
+                    hidden += s["mask"][at + a:at + b, :kv].double()
+                for g in range(h * G, h * G + G):
+                    p = torch.softmax(s["q"][at + a:at + b, g].double() @ k.T / math.sqrt(D) + hidden, -1)
+                    # a row that sees no key is zero
+                    O[at + a:at + b, g] = torch.where(torch.isneginf(hidden).all(-1, keepdim=True), 0.0, p) @ v
+        at += nq
+    return O
+
+
+def _product_exact(case, seed):
+    X, W, bias, R = _product_inputs(case, seed)
+    t = case["type"]
+    if t in ("f32", "f16"):
+        x, w = (X.double(), W.double()) if t == "f32" else (X.half().double(), W.half().double())
+        y = x @ w.T
+    else:
+        q, d, m = _weight_codes(t, W)
+        w = ((q.double() - (8 if t == "q4_0" else 0)) * d.double()[..., None]).reshape(W.shape)
+        xq, xd, raw = _blocks_exact("q8_0", X.view(X.shape[0], -1, 32))
+        y = (xq * xd[..., None]).reshape(X.shape) @ w.T
+        if m is not None:
+            y += _f32(raw * xq.sum(-1)).half().double() @ m.double().T
+    if bias is not None:
+        y += bias.double()
+    if case["act"] == "relu":
+        y = y.clamp(min=0)
+    elif case["act"] == "gelu_erf":
+        y = y * torch.special.ndtr(y)
+    elif case["act"] == "gelu_tanh":
+        y = y * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (y + 0.044715 * y ** 3))
+    elif case["act"] == "silu":
+        y = y * torch.sigmoid(y)
+    return y if R is None else y + R.double()
+
+
+def exact(case, seed):
+    return {"cache": _cache_exact, "attn": _attn_exact, "product": _product_exact}[case["kind"]](case, seed)

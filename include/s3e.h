@@ -246,6 +246,92 @@ int s3e_flash_attn_ext_f16(s3e_ctx *ctx,
                            int64_t D, int64_t Nq, int64_t Nkv, int64_t nh, int64_t B,
                            float scale, float *o);
 
+/* ---- quantized key/value cache --------------------------------------------
+ * What ggml graphs keep between calls in Q4_0 / Q8_0 K and V tensors
+ * (ggml_set_rows into them, ggml_get_rows out of them, ggml_flash_attn_ext on
+ * them with a mask and with more query heads than key/value heads): here one
+ * paged cache in caller memory, in a layout the attention kernel streams.
+ *
+ * The cache is `n_pages` pages of `page` tokens in `data` (device, 16-byte
+ * aligned, s3e_kv_cache_bytes bytes).  Slot p·page + i is token i of page p.
+ * A page holds for each key/value head page/32 chunks of 32 tokens, and a
+ * chunk of head_dim D = 32·NB channels its K words, K scales, V words and V
+ * scales.  A word is eight codes of B = 4 (Q4_0) or 8 (Q8_0) bytes, and each
+ * of 64 lanes has 2·NB words.  K: key 8a + 4t + i of the chunk (a, i < 4,
+ * t < 2) and channels 32b + 8g + j (g < 4, j < 8) are code j of word t·NB + b
+ * of lane 16g + 4a + i.  V: channel 16w + m (m < 16) and key 8g + j are code j
+ * of word w of lane 16g + m.  Words w are stored in pieces of 16/B of them (the
+ * last piece may have fewer): for each piece the 64 lanes' words, lane by
+ * lane.  Code j of a Q4_0 word (0..15, value d·(code − 8)) is bits 4n..4n+3
+ * with n = (j >> 1) + 4·(j & 1); of a Q8_0 word (int8, value d·code) byte j.
+ * Scales are fp16 [NB][32 keys].  A chunk is 36·D (Q4_0) or 68·D bytes.
+ * Memory need not be initialised: only slots that were written are read, and
+ * whatever others hold reaches no result. */
+typedef struct s3e_kv_cache {
+    int32_t type;     /* S3E_TYPE_Q4_0 or S3E_TYPE_Q8_0 */
+    int32_t n_heads;  /* key/value heads */
+    int32_t head_dim; /* D: 32, 64, 96, 128 or 256 */
+    int32_t page;     /* tokens of a page: 32, 64, 128 or 256 */
+    int64_t n_pages;  /* n_pages · page below 2^31 */
+    void *data;       /* device */
+} s3e_kv_cache;
+/* Bytes of `data` (which may still be NULL). */
+int s3e_kv_cache_bytes(const s3e_kv_cache *c, size_t *bytes);
+
+/* Quantise n rows of K and V as they are written: row r, head h of `k` is D
+ * contiguous values at k + r·k_nb[0] + h·k_nb[1] (element strides, none
+ * negative), F32 or F16 by `type` (S3E_TYPE_F32 / S3E_TYPE_F16); `v` likewise.
+ * It goes to slot slots[r] (device, n int32): ggml_set_rows' conversion, Q4_0
+ * as quantize_row_q4_0 (d = max/−8 of the first value of largest magnitude,
+ * code min(15, ⌊x/d + 8.5⌋)), Q8_0 as s3e_quantize_rows.  A block of 32 that
+ * holds an infinity or a NaN reads back as NaN; a scale past fp16 is infinite.
+ * A row whose slot is negative or past the cache is left out; the slots of the
+ * others are distinct (of a slot given twice the contents are unspecified).
+ * Other slots keep their bytes.  Asynchronous on the context's stream; allocates nothing. */
+int s3e_kv_write(s3e_ctx *ctx, const s3e_kv_cache *c, int type, const void *k, const int64_t k_nb[2],
+                 const void *v, const int64_t v_nb[2], const int32_t *slots, int64_t n);
+/* Read n slots back (ggml_get_rows): k and v receive [n][n_heads][D] values of
+ * `type` (16-byte aligned), each scale · code rounded to it once; either may be
+ * NULL.  A slot that is negative or past the cache reads as zeros.
+ * Asynchronous; allocates nothing. */
+int s3e_kv_read(s3e_ctx *ctx, const s3e_kv_cache *c, const int32_t *slots, int64_t n, int type, void *k, void *v);
+
+/* A batch of sequences over one cache.  The arrays are device memory, read
+ * when the kernels run, so a captured call serves growing lengths; the counts
+ * are the host's bounds on them. */
+typedef struct s3e_kv_batch {
+    int64_t n_seq;          /* sequences, 0..65535 */
+    int64_t n_tokens;       /* rows of q and o */
+    int64_t max_q;          /* most query rows of one sequence */
+    int64_t max_kv;         /* most keys of one sequence, at most pages_ld · page */
+    const int32_t *q_start; /* [n_seq + 1]: sequence s has rows q_start[s] .. q_start[s + 1] */
+    const int32_t *kv_len;  /* [n_seq]: its keys, the new rows' own among them once written */
+    const int32_t *pages;   /* [n_seq][pages_ld]: page of its tokens i·page .. (i + 1)·page */
+    int64_t pages_ld;
+} s3e_kv_batch;
+/* Device bytes s3e_kv_attn needs at `ws` for nh query heads and `type` (0: none). */
+int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, int type, size_t *bytes);
+/* O = softmax(scale·Q·Kᵀ + mask)·V over the cache, ggml_flash_attn_ext with
+ * quantized K and V: query head h reads key/value head h / (nh / n_heads).
+ * Q(row, h, d) = q[row·q_nb[0] + h·q_nb[1] + d]; o is [n_tokens][nh][D]
+ * (16-byte aligned), of the same `type`:
+ *   S3E_TYPE_F16  q in fp16, probabilities times V's scales rounded to fp16
+ *                 (fp32 scores, sums and accumulation);
+ *   S3E_TYPE_F32  q and those products as fp16 pairs: fp32 attention to ~1e-6.
+ * causal: row i of a sequence's nq sees keys 0 .. kv_len − nq + i; otherwise
+ * all kv_len of them.  mask (NULL: none): fp16, mask[row·mask_ld + key] is
+ * added for every head, mask_ld at least max_kv; −∞ hides the key.  A hidden
+ * key's scales and codes reach no result, whatever they are, nor does a page
+ * the cache does not have (its keys are hidden).  A row that sees no key is
+ * zero.  Rows outside every sequence are left as they are, and so are rows
+ * of a sequence past max_q; keys past max_kv are not seen.  o may be q itself
+ * (same type, contiguous) but must not overlap it otherwise, nor the cache.
+ * ws: device, 16-byte aligned, ws_bytes of it, this call's own until it has
+ * run; with it the call allocates nothing and can be captured.  Asynchronous. */
+int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_batch *b, int type, const void *q,
+                const int64_t q_nb[2], int64_t nh, float scale, int causal, const uint16_t *mask, int64_t mask_ld,
+                void *o, void *ws, size_t ws_bytes);
+
 /* ---- measurement ---------------------------------------------------------
  * No counterpart in the reference: the rates this GPU reaches, against which
  * the benchmark reads its roofline fractions next to the published peaks.

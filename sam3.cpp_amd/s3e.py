@@ -64,6 +64,30 @@ HIERA_VARIANTS = {
 }
 
 
+def _ptr(buf):
+    return buf.ptr if buf else None
+
+
+class KVCache(ctypes.Structure):
+    """s3e_kv_cache over `data`, a buffer of kv_cache_bytes() bytes (kept alive with it)."""
+    _fields_ = [("type", c_int32), ("n_heads", c_int32), ("head_dim", c_int32), ("page", c_int32),
+                ("n_pages", c_int64), ("data", c_void_p)]
+
+    def __init__(self, ggml_type: int, n_heads: int, head_dim: int, page: int, n_pages: int, data=None):
+        super().__init__(ggml_type, n_heads, head_dim, page, n_pages, _ptr(data))
+        self._data = data
+
+
+class KVBatch(ctypes.Structure):
+    """s3e_kv_batch; q_start, kv_len and pages are device int32 buffers (kept alive with it)."""
+    _fields_ = [("n_seq", c_int64), ("n_tokens", c_int64), ("max_q", c_int64), ("max_kv", c_int64),
+                ("q_start", c_void_p), ("kv_len", c_void_p), ("pages", c_void_p), ("pages_ld", c_int64)]
+
+    def __init__(self, n_seq: int, n_tokens: int, max_q: int, max_kv: int, q_start, kv_len, pages, pages_ld: int):
+        super().__init__(n_seq, n_tokens, max_q, max_kv, _ptr(q_start), _ptr(kv_len), _ptr(pages), pages_ld)
+        self._arrays = (q_start, kv_len, pages)
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built; run __graft_entry__.build() first")
@@ -96,6 +120,12 @@ def _load() -> ctypes.CDLL:
                                        c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_int, c_void_p]),
         "s3e_flash_attn_ext_f16": (c_int, [c_void_p, c_void_p, P64, c_void_p, P64, c_void_p, P64,
                                            c_int64, c_int64, c_int64, c_int64, c_int64, c_float, c_void_p]),
+        "s3e_kv_cache_bytes": (c_int, [POINTER(KVCache), POINTER(c_size_t)]),
+        "s3e_kv_write": (c_int, [c_void_p, POINTER(KVCache), c_int, c_void_p, P64, c_void_p, P64, c_void_p, c_int64]),
+        "s3e_kv_read": (c_int, [c_void_p, POINTER(KVCache), c_void_p, c_int64, c_int, c_void_p, c_void_p]),
+        "s3e_kv_attn_workspace": (c_int, [POINTER(KVCache), POINTER(KVBatch), c_int64, c_int, POINTER(c_size_t)]),
+        "s3e_kv_attn": (c_int, [c_void_p, POINTER(KVCache), POINTER(KVBatch), c_int, c_void_p, P64, c_int64, c_float,
+                                c_int, c_void_p, c_int64, c_void_p, c_void_p, c_size_t]),
         "s3e_probe_stream": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_size_t]),
         "s3e_probe_mfma": (c_int, [c_void_p, c_int, c_int64, c_int]),
         "s3e_model_load": (c_int, [c_void_p, c_char_p, POINTER(c_void_p)]),
@@ -138,7 +168,8 @@ DECLARED = [
     "s3e_last_error", "s3e_abi_version", "s3e_ctx_create", "s3e_ctx_destroy", "s3e_ctx_sync", "s3e_ctx_stream",
     "s3e_malloc", "s3e_free", "s3e_memcpy_h2d", "s3e_memcpy_d2h", "s3e_weight_upload", "s3e_weight_free",
     "s3e_weight_info", "s3e_mul_mat", "s3e_mul_mat_noalloc", "s3e_mul_mat_q", "s3e_mul_mat_q_f6", "s3e_mul_mat_q_batch", "s3e_quantize_rows", "s3e_layer_norm", "s3e_copy",
-    "s3e_flash_attn_ext", "s3e_flash_attn_ext_f16", "s3e_probe_stream", "s3e_probe_mfma", "s3e_model_load",
+    "s3e_flash_attn_ext", "s3e_flash_attn_ext_f16", "s3e_kv_cache_bytes", "s3e_kv_write", "s3e_kv_read",
+    "s3e_kv_attn_workspace", "s3e_kv_attn", "s3e_probe_stream", "s3e_probe_mfma", "s3e_model_load",
     "s3e_model_free", "s3e_model_hparams", "s3e_state_create", "s3e_state_create_sized", "s3e_state_free", "s3e_encode_chw",
     "s3e_encode_chw_host", "s3e_encode_image_u8", "s3e_preprocess_image", "s3e_vit_prefix", "s3e_vit_block", "s3e_vit_block_stage", "s3e_vit_prefix_stage", "s3e_encode_vit_chw", "s3e_model_tensor_get", "s3e_run_neck", "s3e_hiera_block", "s3e_model_type", "s3e_mem_attn_dims", "s3e_mem_attn",
     "s3e_state_tensor_info",
@@ -201,6 +232,20 @@ def synth_write_sam2(path: str, variant: str = "hiera_t", *, img_size=1024, ftyp
     cfg.std = -abs(std) if random_affine else abs(std)
     cfg.mem_attn_layers = int(mem_attn_layers)
     check(LIB.s3e_synth_write_sam2(path.encode(), ctypes.byref(cfg)), "s3e_synth_write_sam2")
+
+
+def kv_cache_bytes(cache: KVCache) -> int:
+    n = c_size_t()
+    check(LIB.s3e_kv_cache_bytes(ctypes.byref(cache), ctypes.byref(n)), "s3e_kv_cache_bytes")
+    return n.value
+
+
+def kv_attn_workspace(cache: KVCache, batch: KVBatch, nh: int, ggml_type: int) -> int:
+    """Device bytes Context.kv_attn needs as its workspace."""
+    n = c_size_t()
+    check(LIB.s3e_kv_attn_workspace(ctypes.byref(cache), ctypes.byref(batch), nh, ggml_type, ctypes.byref(n)),
+          "s3e_kv_attn_workspace")
+    return n.value
 
 
 def act_scale_elems(M: int, K: int) -> int:
@@ -325,6 +370,25 @@ class Context:
 
     def mul_mat(self, w: Weight, X: DeviceBuffer, M: int, Y: DeviceBuffer, bias: DeviceBuffer | None = None):
         check(LIB.s3e_mul_mat(self.handle, w.handle, X.ptr, M, bias.ptr if bias else None, Y.ptr), "s3e_mul_mat")
+
+    def kv_write(self, cache: KVCache, ggml_type: int, k: DeviceBuffer, k_nb, v: DeviceBuffer, v_nb,
+                 slots: DeviceBuffer, n: int):
+        """Rows of K and V (element strides: token, head) into the cache's slots."""
+        check(LIB.s3e_kv_write(self.handle, ctypes.byref(cache), ggml_type, k.ptr, (c_int64 * 2)(*k_nb), v.ptr,
+                               (c_int64 * 2)(*v_nb), slots.ptr, n), "s3e_kv_write")
+
+    def kv_read(self, cache: KVCache, slots: DeviceBuffer, n: int, ggml_type: int, k: DeviceBuffer | None,
+                v: DeviceBuffer | None):
+        check(LIB.s3e_kv_read(self.handle, ctypes.byref(cache), slots.ptr, n, ggml_type, _ptr(k), _ptr(v)),
+              "s3e_kv_read")
+
+    def kv_attn(self, cache: KVCache, batch: KVBatch, ggml_type: int, q: DeviceBuffer, q_nb, nh: int, scale: float,
+                o: DeviceBuffer, ws: DeviceBuffer | None = None, *, causal: bool = False,
+                mask: DeviceBuffer | None = None, mask_ld: int = 0):
+        """Attention of the batch's queries (element strides: token, head) over the cache."""
+        check(LIB.s3e_kv_attn(self.handle, ctypes.byref(cache), ctypes.byref(batch), ggml_type, q.ptr,
+                              (c_int64 * 2)(*q_nb), nh, scale, int(causal), _ptr(mask), mask_ld, o.ptr, _ptr(ws),
+                              ws.nbytes if ws else 0), "s3e_kv_attn")
 
     def quantize_rows(self, vdt: int, X: DeviceBuffer, M: int, K: int, qs: DeviceBuffer,
                       d: DeviceBuffer | None, s: DeviceBuffer | None):

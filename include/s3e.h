@@ -118,6 +118,24 @@ int s3e_weight_info(const s3e_weight *w, int64_t out[4]);
 int s3e_mul_mat(s3e_ctx *ctx, const s3e_weight *w, const float *X, int64_t M,
                 const float *bias, float *Y);
 
+/* Y = act(ggml_mul_mat(W, X) + bias) + residual in the product's epilogue:
+ * ggml_add, an activation and a second ggml_add behind s3e_mul_mat, whose
+ * conversion of X and products these are (sam3.cpp:3779-3780, 3792-3796 and
+ * the residual adds around them).  X is M rows of K f32 and Y of N f32
+ * (device); bias (N f32) and residual (M rows of N f32, which may be Y itself)
+ * may be NULL.  act is computed in fp32: RELU x > 0 ? x : 0, GELU_ERF
+ * ggml_gelu_erf, GELU_TANH ggml_gelu's formula (not its fp16 table), SILU
+ * x / (1 + e^-x).  Y overlaps neither X nor bias.  M = 0 succeeds and writes
+ * nothing; at most 262 140 rows, whose converted X (as s3e_mul_mat) stays below 2 GiB.
+ * ws: device, 16-byte aligned, at least s3e_mul_mat_act_workspace bytes (0:
+ * may be NULL), this call's own until it has run.  Asynchronous on the
+ * context's stream; allocates nothing, waits for nothing, and can be captured:
+ * a captured call gives the eager one's results. */
+enum s3e_act { S3E_ACT_NONE = 0, S3E_ACT_RELU = 1, S3E_ACT_GELU_ERF = 2, S3E_ACT_GELU_TANH = 3, S3E_ACT_SILU = 4 };
+int s3e_mul_mat_act_workspace(const s3e_weight *w, int64_t M, size_t *bytes);
+int s3e_mul_mat_act(s3e_ctx *ctx, const s3e_weight *w, const float *X, int64_t M, const float *bias, int act,
+                    const float *residual, float *Y, void *ws, size_t ws_bytes);
+
 /* No counterpart in the reference: s3e_mul_mat for callers that cannot
  * allocate device memory (code under HIP graph capture, serving loops that
  * forbid hipMalloc).  Same arguments and results; X is converted into a

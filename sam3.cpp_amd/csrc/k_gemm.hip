@@ -619,7 +619,7 @@ __device__ __forceinline__ void epilogue(const GemmParams &p, const float *Ct, i
         const int gn = n0 + 4 * f;
         const bool vec = (p.N % 4) == 0 && gn + 3 < p.N;
         constexpr int RPT = BM / (NT_ / 32);  // rows per thread
-        if constexpr (EPI == EPI_RESID) {
+        if constexpr (EPI == EPI_RESID || EPI == EPI_FUSED) {
             if (vec) {
                 // the bias, and every residual row of this thread, are loaded
                 // before the first store: y and bias may alias as far as the
@@ -627,12 +627,13 @@ __device__ __forceinline__ void epilogue(const GemmParams &p, const float *Ct, i
                 // for that store
                 const float4 bb = e.bias ? *(const float4 *)(e.bias + gn) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float bj[4] = {bb.x, bb.y, bb.z, bb.w};
+                const float *const rp = EPI == EPI_RESID ? e.y : e.resid;
                 float4 res[RPT];
 #pragma unroll
                 for (int k = 0; k < RPT; k++) {
                     const int gm = m0 + (t >> 5) + k * (NT_ / 32);
-                    res[k] = gm < p.M ? *(const float4 *)(e.y + (int64_t)gm * e.ldy + gn)
-                                      : make_float4(0.f, 0.f, 0.f, 0.f);
+                    res[k] = gm < p.M && (EPI == EPI_RESID || rp) ? *(const float4 *)(rp + (int64_t)gm * e.ldy + gn)
+                                                                  : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
                 for (int k = 0; k < RPT; k++) {
@@ -643,6 +644,14 @@ __device__ __forceinline__ void epilogue(const GemmParams &p, const float *Ct, i
                     if (e.bias) {
 #pragma unroll
                         for (int j = 0; j < 4; j++) v[j] = __fadd_rn(v[j], bj[j]);
+                    }
+                    if constexpr (EPI == EPI_FUSED) {
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = act_f32(e.act, v[j]);
+                        if (!rp) {  // (−0 stays −0)
+                            *(float4 *)(e.y + (int64_t)gm * e.ldy + gn) = make_float4(v[0], v[1], v[2], v[3]);
+                            continue;
+                        }
                     }
                     *(float4 *)(e.y + (int64_t)gm * e.ldy + gn) =
                         make_float4(__fadd_rn(res[k].x, v[0]), __fadd_rn(res[k].y, v[1]),
@@ -713,7 +722,10 @@ __device__ __forceinline__ void epilogue(const GemmParams &p, const float *Ct, i
             }
             for (int j = 0; j < 4 && gn + j < p.N; j++) {
                 if constexpr (EPI == EPI_RESID) y[j] = __fadd_rn(y[j], v[j]);
-                else y[j] = v[j];
+                else if constexpr (EPI == EPI_FUSED) {
+                    const float a = act_f32(e.act, v[j]);
+                    y[j] = e.resid ? __fadd_rn(e.resid[(int64_t)gm * e.ldy + gn + j], a) : a;
+                } else y[j] = v[j];
             }
         }
     }
@@ -1104,7 +1116,7 @@ __global__ __launch_bounds__(64 * WAVES, RING ? 1 : (WAVES == 4 ? 3 : 256 / BM))
             }
     __syncthreads();
 
-    if constexpr (EPI == EPI_F32 || EPI == EPI_RESID) {
+    if constexpr (EPI == EPI_F32 || EPI == EPI_RESID || EPI == EPI_FUSED) {
         if (p.ksplit > 1) {
             // raw partial tile of this K range; the reduction adds bias / residual
             GemmParams q = p;
@@ -1296,7 +1308,7 @@ __global__ __launch_bounds__(256, 3) void k_gemm_f6(GemmParams p) {
             Ct[row * CLD + wn * 64 + 32 * n + lr] = acc[n][r] * 0.5f;  // the doubled scale products
         }
     __syncthreads();
-    if constexpr (EPI == EPI_F32 || EPI == EPI_RESID) {
+    if constexpr (EPI == EPI_F32 || EPI == EPI_RESID || EPI == EPI_FUSED) {
         if (p.ksplit > 1) {
             GemmParams q = p;
             q.e.y = p.part + (int64_t)kpart * p.M * p.N;
@@ -1310,11 +1322,12 @@ __global__ __launch_bounds__(256, 3) void k_gemm_f6(GemmParams p) {
 }
 
 // y = Σ_k part[k] (+ bias) for EPI_F32, y += Σ_k part[k] (+ bias) for
-// EPI_RESID, the ranges summed in order (the result does not depend on the
+// EPI_RESID (resid is y), y = act(Σ_k part[k] (+ bias)) (+ resid) for
+// EPI_FUSED, the ranges summed in order (the result does not depend on the
 // schedule).  One thread per 4 consecutive outputs of a row.
 __global__ __launch_bounds__(256) void k_gemm_reduce(const float *__restrict__ part, int ks, int M, int N,
                                                      const float *__restrict__ bias, float *y, int64_t ldy,
-                                                     int resid) {
+                                                     const float *resid, int act) {
     const uint32_t i = blockIdx.x * 256 + threadIdx.x;
     const uint32_t n4 = (uint32_t)N / 4;
     if (i >= (uint32_t)M * n4) return;
@@ -1335,9 +1348,10 @@ __global__ __launch_bounds__(256) void k_gemm_reduce(const float *__restrict__ p
         v.z = __fadd_rn(v.z, bias[c + 2]);
         v.w = __fadd_rn(v.w, bias[c + 3]);
     }
+    if (act) v = make_float4(act_f32(act, v.x), act_f32(act, v.y), act_f32(act, v.z), act_f32(act, v.w));
     float4 *o = (float4 *)(y + (int64_t)r * ldy + c);
     if (resid) {
-        const float4 x = *o;
+        const float4 x = *(const float4 *)(resid + (int64_t)r * ldy + c);
         v = make_float4(__fadd_rn(x.x, v.x), __fadd_rn(x.y, v.y), __fadd_rn(x.z, v.z), __fadd_rn(x.w, v.w));
     }
     *o = v;
@@ -1355,6 +1369,9 @@ hipError_t dispatch_epi(Epi epi, const GemmParams &p, hipStream_t st) {
     switch (epi) {
         case EPI_F32: return launch_one<WK, EPI_F32, 64, WAVES>(p, st);
         case EPI_RESID: return launch_one<WK, EPI_RESID, 64, WAVES>(p, st);
+        case EPI_FUSED:
+            if constexpr (WK != WK_F16X3) return launch_one<WK, EPI_FUSED, 64, WAVES>(p, st);  // (uploaded weights)
+            break;
         case EPI_POS: return launch_one<WK, EPI_POS, 64, WAVES>(p, st);
         case EPI_GELU: return launch_one<WK, EPI_GELU, 64, WAVES>(p, st);
         case EPI_QKV: return launch_one<WK, EPI_QKV, 64, WAVES>(p, st);
@@ -1389,11 +1406,12 @@ hipError_t dispatch_waves(Epi epi, GemmParams &p, hipStream_t st) {
     if constexpr (WK == WK_F16) {
         const int64_t t128 = (int64_t)(p.M + 127) / 128 * p.tiles_n;
         if (p.ksplit == 1 && (t128 >= F16_WIDE_MIN_TILES || (p.e.lone && f16_wide_lone(t128))) && p.a_kbytes >= 2 * F16_WIDE_MIN_K &&
-            (epi == EPI_F32 || epi == EPI_GELU || epi == EPI_QKV || epi == EPI_HQKV || epi == EPI_DECONV)) {
+            (epi == EPI_F32 || epi == EPI_FUSED || epi == EPI_GELU || epi == EPI_QKV || epi == EPI_HQKV || epi == EPI_DECONV)) {
             p.tiles_m = (p.M + 127) / 128;
             p.ntiles = p.tiles_m * p.tiles_n;
             switch (epi) {
                 case EPI_F32: return launch_one<WK, EPI_F32, 128, 4>(p, st);
+                case EPI_FUSED: return launch_one<WK, EPI_FUSED, 128, 4>(p, st);
                 case EPI_GELU: return launch_one<WK, EPI_GELU, 128, 4>(p, st);
                 case EPI_QKV: return launch_one<WK, EPI_QKV, 128, 4>(p, st);
                 case EPI_DECONV: return launch_one<WK, EPI_DECONV, 128, 4>(p, st);
@@ -1409,6 +1427,9 @@ hipError_t dispatch_waves(Epi epi, GemmParams &p, hipStream_t st) {
         if (p.e.lone && p.ntiles * p.ksplit <= 256) {
             if (epi == EPI_F32) return launch_one<WK, EPI_F32, BM, 4, DEEP_RING>(p, st);
             if (epi == EPI_RESID) return launch_one<WK, EPI_RESID, BM, 4, DEEP_RING>(p, st);
+            if constexpr (WK == WK_F16) {
+                if (epi == EPI_FUSED) return launch_one<WK, EPI_FUSED, BM, 4, DEEP_RING>(p, st);
+            }
         }
     }
     // 4-wave work-groups (three per CU, 4-12% faster on the SAM 3 shapes)
@@ -1495,7 +1516,7 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
     p.M = (int)M;
     p.N = (int)w.N;
     p.ksplit = 1;
-    if ((epi == EPI_F32 || epi == EPI_RESID) && ea.ws && ea.ldy % 4 == 0) {
+    if ((epi == EPI_F32 || epi == EPI_RESID || epi == EPI_FUSED) && ea.ws && ea.ldy % 4 == 0) {
         const int ks = splitk_of(w, M, ea.frame);
         if (ks > 1 && (int64_t)ks * M * w.N <= ea.ws_cap) {
             p.ksplit = ks;
@@ -1542,6 +1563,7 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
         switch (epi) {
             case EPI_F32: hipLaunchKernelGGL(k_gemm_f6<EPI_F32>, dim3(grid), dim3(256), 0, st, p); break;
             case EPI_RESID: hipLaunchKernelGGL(k_gemm_f6<EPI_RESID>, dim3(grid), dim3(256), 0, st, p); break;
+            case EPI_FUSED: hipLaunchKernelGGL(k_gemm_f6<EPI_FUSED>, dim3(grid), dim3(256), 0, st, p); break;
             case EPI_GELU: hipLaunchKernelGGL(k_gemm_f6<EPI_GELU>, dim3(grid), dim3(256), 0, st, p); break;
             case EPI_QKV: hipLaunchKernelGGL(k_gemm_f6<EPI_QKV>, dim3(grid), dim3(256), 0, st, p); break;
             default: return hipErrorInvalidValue;
@@ -1550,7 +1572,9 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
         if (e == hipSuccess && p.ksplit > 1) {
             const int64_t n = M * (w.N / 4);
             hipLaunchKernelGGL(k_gemm_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p.part, p.ksplit,
-                               (int)M, (int)w.N, ea.bias, ea.y, ea.ldy, epi == EPI_RESID ? 1 : 0);
+                               (int)M, (int)w.N, ea.bias, ea.y, ea.ldy,
+                               epi == EPI_RESID ? ea.y : (epi == EPI_FUSED ? ea.resid : nullptr),
+                               epi == EPI_FUSED ? ea.act : 0);
             e = hipGetLastError();
         }
         return e;
@@ -1571,7 +1595,9 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
     if (e == hipSuccess && p.ksplit > 1) {
         const int64_t n = M * (w.N / 4);
         hipLaunchKernelGGL(k_gemm_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p.part, p.ksplit,
-                           (int)M, (int)w.N, ea.bias, ea.y, ea.ldy, epi == EPI_RESID ? 1 : 0);
+                           (int)M, (int)w.N, ea.bias, ea.y, ea.ldy,
+                               epi == EPI_RESID ? ea.y : (epi == EPI_FUSED ? ea.resid : nullptr),
+                               epi == EPI_FUSED ? ea.act : 0);
         e = hipGetLastError();
     }
     return e;

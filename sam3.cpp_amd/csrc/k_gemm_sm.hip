@@ -319,7 +319,10 @@ __global__ __launch_bounds__(64 * SM_WAVES, 2) void k_gemm_sm(SmArgs p) {
                 for (int w = 1; w < KS; w++) v += red[st * KS + w][row][col];
                 v *= kScale;
                 if (G.bias) v += G.bias[gn];
-                G.y[(int64_t)(r0 + row) * G.ldy + gn] = v;
+                const int64_t at = (int64_t)(r0 + row) * G.ldy + gn;
+                if (p.act) v = act_f32(p.act, v);
+                if (p.resid) v += p.resid[at];
+                G.y[at] = v;
             }
             return;
         }
@@ -337,12 +340,12 @@ __global__ __launch_bounds__(64 * SM_WAVES, 2) void k_gemm_sm(SmArgs p) {
     }
 }
 
-// Y = scale · Σ_k part[k] + bias over the kg ≤ SM_KG_MAX partial sums of a
+// Y = act(scale · Σ_k part[k] + bias) + resid over the kg ≤ SM_KG_MAX partial sums of a
 // split small-M product, added in index order (one thread per output; the kg
 // loads are all issued before the first add).
 __global__ __launch_bounds__(256) void k_sm_reduce(const float *__restrict__ part, int kg, int64_t mn, int N,
-                                                  float scale, const float *__restrict__ bias, float *__restrict__ y,
-                                                  int64_t ldy) {
+                                                  float scale, const float *__restrict__ bias, float *y, int64_t ldy,
+                                                  int act, const float *resid) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= mn) return;
     float pv[SM_KG_MAX];
@@ -355,6 +358,8 @@ __global__ __launch_bounds__(256) void k_sm_reduce(const float *__restrict__ par
     const int col = (int)(i - row * N);
     v *= scale;
     if (bias) v += bias[col];
+    if (act) v = act_f32(act, v);
+    if (resid) v += resid[row * ldy + col];
     y[row * ldy + col] = v;
 }
 
@@ -711,7 +716,7 @@ hipError_t launch_gemm_sm(WKind kind, const SmArgs &a, int wgs, int ks, hipStrea
     const int64_t mn = (int64_t)a.M * g.N;
     const float scale = kind == WK_F16 ? 1.0f : 0.5f;  // the quantized scale products are doubled
     hipLaunchKernelGGL(k_sm_reduce, dim3((unsigned)((mn + 255) / 256)), dim3(256), 0, st, (const float *)a.part, a.kg,
-                       mn, g.N, scale, g.bias, g.y, g.ldy);
+                       mn, g.N, scale, g.bias, g.y, g.ldy, a.act, a.resid);
     return hipGetLastError();
 }
 

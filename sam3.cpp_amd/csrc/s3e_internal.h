@@ -163,6 +163,7 @@ enum Epi : int {
     EPI_ACT = 6,     // act = acc + bias                     (conv → next conv)
     EPI_HQKV = 7,    // Hiera: Q/K/Vᵀ in window order (padded grid, heads padded to hdp), fp16
                      // (hi, lo); with qpool, Q as f32 rows into y for the pooling pass
+    EPI_FUSED = 8,   // y = act(acc + bias) + resid          (s3e_mul_mat_act)
 };
 
 struct EpiArgs {
@@ -175,11 +176,14 @@ struct EpiArgs {
     // a product of an encode or a memory-attention pass: the K ranges of those
     // (splitk_of)
     bool frame = false;
-    // EPI_F32 / EPI_RESID: workspace for a split over K (gemm_splitk_floats
+    // EPI_F32 / EPI_RESID / EPI_FUSED: workspace for a split over K (gemm_splitk_floats
     // floats); null: never split
     float *ws = nullptr;
     int64_t ws_cap = 0;
     Act out;                     // EPI_GELU
+    // EPI_FUSED: an s3e_act, and rows of ldy to add (may be y) or null
+    int act = 0;
+    const float *resid = nullptr;
     // EPI_POS
     const float *pos = nullptr;  // [pg][pg][E]
     int pos_grid = 0;
@@ -311,6 +315,10 @@ struct SmArgs {
     // k_gemm_sm, one product: X as f32 rows of one.ldx, converted in the kernel
     // (one.x, xd and xs are then unused)
     const float *x32 = nullptr;
+    // k_gemm_sm, one product: y = act(W·x + bias) + resid, as EPI_FUSED (rows
+    // of one.ldy)
+    int act = 0;
+    const float *resid = nullptr;
 };
 
 // ---- kernel launchers (k_*.hip) ----
@@ -450,6 +458,19 @@ __device__ __forceinline__ float gelu_erf(float x) {
     const float E = t * P * e;
     const float w = (x >= 0.f) ? 2.0f - E : E;
     return 0.5f * x * w;
+}
+
+// An s3e_act of v in fp32 (uniform over the launch).  The tanh form and SiLU
+// are x / (1 + e^−z): z = 2·√(2/π)·(x + 0.044715·x³), and x.
+__device__ __forceinline__ float act_f32(int act, float x) {
+    switch (act) {
+        case S3E_ACT_RELU: return x > 0.f ? x : 0.f;
+        case S3E_ACT_GELU_ERF: return gelu_erf(x);
+        case S3E_ACT_GELU_TANH:
+            return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * __builtin_fmaf(x * x, -0.10294324f, -2.30220819f)));
+        case S3E_ACT_SILU: return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -1.4426950408889634f));
+        default: return x;
+    }
 }
 
 // ggml_gelu of the fp16 value xh, as ggml's fp16 table holds it, without

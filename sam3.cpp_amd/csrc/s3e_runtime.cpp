@@ -701,6 +701,134 @@ extern "C" int s3e_mul_mat(s3e_ctx *ctx, const s3e_weight *w, const float *X, in
     return S3E_OK;
 } S3E_CATCH("s3e_mul_mat")
 
+// s3e_mul_mat_act's workspace: [X in the product's format][d][s][partial sums],
+// or without conversion (rows converted by the kernel, F32) the sums alone.
+namespace {
+struct ActPlan {
+    Act a;
+    bool small = false, x32 = false;
+    int kg = 1;                 // K ranges of a small product
+    size_t vb = 0, sb = 0;      // bytes of the values and of one scale plane
+    int64_t parts = 0;          // floats of partial sums
+    size_t bytes() const { return vb + 2 * sb + (size_t)parts * 4; }
+};
+ActPlan plan_act(const Weight &W, int64_t M) {
+    ActPlan p;
+    p.small = sm_eligible(W, M);
+    p.x32 = sm_converts(W, M);
+    p.a.ld = W.K;
+    p.a.kind = p.small ? act_kind_for(W.kind) : act_kind_gemm(W);
+    p.a.mp = round_up(M, ROW_PAD);
+    if (p.a.kind != A_F32 && !p.x32) {
+        const bool f16 = p.a.kind == A_F16;
+        p.vb = (size_t)(p.a.mp * W.K) * (f16 ? 4 : 3) / 2;  // fp6 pairs take 1.5 bytes, Q8 codes 1
+        p.sb = f16 ? 0 : (size_t)(p.a.mp * (round_up(W.K, 128) / QK)) * 2;
+    }
+    if (p.small) {
+        p.kg = sm_kgroups(W);
+        if (p.kg > 1) p.parts = p.kg * M * W.N;
+    } else {
+        p.parts = gemm_splitk_floats(W, M, false);
+    }
+    return p;
+}
+
+// What the kernels reach: rows of X in the product's format (buffer loads take
+// byte offsets below 2^31), and rows over the grid of the conversion.
+int check_act(const char *fn, const s3e_weight *w, int64_t M) {
+    if (!w) { set_error("%s: NULL argument", fn); return S3E_ERR_INVALID; }
+    if (M < 0) { set_error("%s: negative M", fn); return S3E_ERR_INVALID; }
+    const Weight &W = w->w;
+    if (W.K % 32 != 0) { set_error("%s: K=%lld is not a multiple of 32", fn, (long long)W.K); return S3E_ERR_UNSUPPORTED; }
+    const int64_t row = W.kind == WK_F32 ? 4 * W.K : (W.kind == WK_F16 ? 2 * W.K : 3 * W.K / 2);
+    if (M > 4 * 65535 || round_up(M, ROW_PAD) > INT32_MAX / row || M > INT32_MAX / W.N) {
+        set_error("%s: %lld rows of K=%lld and N=%lld are too many", fn, (long long)M, (long long)W.K, (long long)W.N);
+        return S3E_ERR_UNSUPPORTED;
+    }
+    return S3E_OK;
+}
+}  // namespace
+
+extern "C" int s3e_mul_mat_act_workspace(const s3e_weight *w, int64_t M, size_t *bytes) try {
+    if (!bytes) { set_error("s3e_mul_mat_act_workspace: NULL argument"); return S3E_ERR_INVALID; }
+    const int rc = check_act("s3e_mul_mat_act_workspace", w, M);
+    if (rc == S3E_OK) *bytes = M ? plan_act(w->w, M).bytes() : 0;
+    return rc;
+} S3E_CATCH("s3e_mul_mat_act_workspace")
+
+extern "C" int s3e_mul_mat_act(s3e_ctx *ctx, const s3e_weight *w, const float *X, int64_t M, const float *bias, int act,
+                               const float *residual, float *Y, void *ws, size_t ws_bytes) try {
+    const char *fn = "s3e_mul_mat_act";
+    if (!ctx || !w || !X || !Y) { set_error("%s: NULL argument", fn); return S3E_ERR_INVALID; }
+    const int rc = check_act(fn, w, M);
+    if (rc != S3E_OK) return rc;
+    if (act < S3E_ACT_NONE || act > S3E_ACT_SILU) { set_error("%s: no activation %d", fn, act); return S3E_ERR_INVALID; }
+    const Weight &W = w->w;
+    if (w->ctx->device != ctx->device) { set_error("%s: the weight lies on another device", fn); return S3E_ERR_INVALID; }
+    if (((uintptr_t)X | (uintptr_t)Y | (uintptr_t)bias | (uintptr_t)residual) % 4 != 0) {
+        set_error("%s: a pointer is not 4-byte aligned", fn);
+        return S3E_ERR_INVALID;
+    }
+    if (M == 0) return S3E_OK;
+    const size_t xb = (size_t)(M * W.K) * 4, yb = (size_t)(M * W.N) * 4;
+    if (overlap(Y, yb, X, xb) || (bias && overlap(Y, yb, bias, (size_t)W.N * 4)) ||
+        (residual && residual != Y && overlap(Y, yb, residual, yb))) {
+        set_error("%s: Y overlaps X, the bias or part of the residual", fn);
+        return S3E_ERR_INVALID;
+    }
+    ActPlan p = plan_act(W, M);
+    const size_t need = p.bytes();
+    if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16 != 0)) {
+        set_error("%s: needs %zu bytes of 16-byte aligned workspace, has %zu", fn, need, ws ? ws_bytes : (size_t)0);
+        return S3E_ERR_INVALID;
+    }
+    if (need && (overlap(ws, need, X, xb) || overlap(ws, need, Y, yb) || (residual && overlap(ws, need, residual, yb)) ||
+                 (bias && overlap(ws, need, bias, (size_t)W.N * 4)))) {
+        set_error("%s: the workspace overlaps X, Y, the bias or the residual", fn);
+        return S3E_ERR_INVALID;
+    }
+    HIP_TRY(hipSetDevice(ctx->device));
+    hipStream_t st = ctx->stream;
+    uint8_t *base = (uint8_t *)ws;
+    float *const parts = p.parts ? (float *)(base + p.vb + 2 * p.sb) : nullptr;
+    if (p.vb) {
+        // rows past M of the values and scale planes are never written: they
+        // only reach output rows past M, which no kernel stores
+        p.a.x = base;
+        p.a.d = (uint16_t *)(base + p.vb);
+        p.a.s = (uint16_t *)(base + p.vb + p.sb);
+        HIP_TRY(launch_rows_quant(p.a.kind, X, M, W.K, p.a, st));
+    } else {
+        p.a.x = (void *)X;
+    }
+    if (p.small) {
+        const uint8_t *wsm = nullptr;
+        HIP_TRY(sm_weights(w, st, &wsm));  // made when the weight was uploaded
+        SmArgs sa;
+        sa.one = sm_desc(W, wsm, p.a, bias, Y, 0);
+        sa.M = (int)M;
+        sa.x32 = p.x32 ? X : nullptr;
+        sa.kg = p.kg;
+        sa.part = parts;
+        sa.rt = (SM_ROW_TILES && M > 32) ? 2 : 1;
+        sa.act = act;
+        sa.resid = residual;
+        HIP_TRY(launch_gemm_sm(W.kind, sa, sm_wgs(W.N, SM_KS) * sa.kg * sa.rt, SM_KS, st));
+        return S3E_OK;
+    }
+    EpiArgs ea;
+    ea.bias = bias;
+    ea.y = Y;
+    ea.ldy = W.N;
+    ea.act = act;
+    ea.resid = residual;
+    ea.lone = true;
+    ea.ws = parts;
+    ea.ws_cap = p.parts;
+    HIP_TRY(launch_gemm(W, p.a, M, EPI_FUSED, ea, st));
+    return S3E_OK;
+} S3E_CATCH("s3e_mul_mat_act")
+
 extern "C" int s3e_mul_mat_q_f6(s3e_ctx *ctx, const s3e_weight *w, const void *xq, const uint16_t *d, int64_t M,
                                 const float *bias, float *Y) try {
     if (!ctx || !w || !xq || !d || !Y) { set_error("s3e_mul_mat_q_f6: NULL argument"); return S3E_ERR_INVALID; }

@@ -20,6 +20,7 @@ LIB_PATH = os.environ.get("S3E_LIB_PATH", os.path.join(HERE, "libs3e.so"))
 TYPE_F32, TYPE_F16, TYPE_Q4_0, TYPE_Q4_1, TYPE_Q8_0, TYPE_Q8_1 = 0, 1, 2, 3, 8, 9
 TYPE_Q8_0_F6X2 = 64  # the Q8_0 codes split into two fp6 halves (engine layout)
 PREC_DEFAULT, PREC_F32 = 0, 1
+ACTS = {"none": 0, "relu": 1, "gelu_erf": 2, "gelu_tanh": 3, "silu": 4}  # enum s3e_act
 FTYPE_BY_NAME = {"f32": 0, "f16": 1, "q4_0": 2, "q4_1": 3, "q8_0": 8}
 
 
@@ -108,6 +109,9 @@ def _load() -> ctypes.CDLL:
         "s3e_weight_free": (None, [c_void_p]),
         "s3e_weight_info": (c_int, [c_void_p, P64]),
         "s3e_mul_mat": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+        "s3e_mul_mat_act_workspace": (c_int, [c_void_p, c_int64, POINTER(c_size_t)]),
+        "s3e_mul_mat_act": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                                    c_size_t]),
         "s3e_mul_mat_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
         "s3e_quantize_rows": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
         "s3e_layer_norm": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
@@ -167,7 +171,7 @@ LIB = _load()
 DECLARED = [
     "s3e_last_error", "s3e_abi_version", "s3e_ctx_create", "s3e_ctx_destroy", "s3e_ctx_sync", "s3e_ctx_stream",
     "s3e_malloc", "s3e_free", "s3e_memcpy_h2d", "s3e_memcpy_d2h", "s3e_weight_upload", "s3e_weight_free",
-    "s3e_weight_info", "s3e_mul_mat", "s3e_mul_mat_noalloc", "s3e_mul_mat_q", "s3e_mul_mat_q_f6", "s3e_mul_mat_q_batch", "s3e_quantize_rows", "s3e_layer_norm", "s3e_copy",
+    "s3e_weight_info", "s3e_mul_mat", "s3e_mul_mat_act_workspace", "s3e_mul_mat_act", "s3e_mul_mat_noalloc", "s3e_mul_mat_q", "s3e_mul_mat_q_f6", "s3e_mul_mat_q_batch", "s3e_quantize_rows", "s3e_layer_norm", "s3e_copy",
     "s3e_flash_attn_ext", "s3e_flash_attn_ext_f16", "s3e_kv_cache_bytes", "s3e_kv_write", "s3e_kv_read",
     "s3e_kv_attn_workspace", "s3e_kv_attn", "s3e_probe_stream", "s3e_probe_mfma", "s3e_model_load",
     "s3e_model_free", "s3e_model_hparams", "s3e_state_create", "s3e_state_create_sized", "s3e_state_free", "s3e_encode_chw",
@@ -245,6 +249,13 @@ def kv_attn_workspace(cache: KVCache, batch: KVBatch, nh: int, ggml_type: int) -
     n = c_size_t()
     check(LIB.s3e_kv_attn_workspace(ctypes.byref(cache), ctypes.byref(batch), nh, ggml_type, ctypes.byref(n)),
           "s3e_kv_attn_workspace")
+    return n.value
+
+
+def mul_mat_act_workspace(w: "Weight", M: int) -> int:
+    """Device bytes Context.mul_mat_act needs as its workspace."""
+    n = c_size_t()
+    check(LIB.s3e_mul_mat_act_workspace(w.handle, M, ctypes.byref(n)), "s3e_mul_mat_act_workspace")
     return n.value
 
 
@@ -370,6 +381,12 @@ class Context:
 
     def mul_mat(self, w: Weight, X: DeviceBuffer, M: int, Y: DeviceBuffer, bias: DeviceBuffer | None = None):
         check(LIB.s3e_mul_mat(self.handle, w.handle, X.ptr, M, bias.ptr if bias else None, Y.ptr), "s3e_mul_mat")
+
+    def mul_mat_act(self, w: Weight, X: DeviceBuffer, M: int, Y: DeviceBuffer, ws: DeviceBuffer | None = None, *,
+                    bias: DeviceBuffer | None = None, act: str = "none", residual: DeviceBuffer | None = None):
+        """Y = act(W X + bias) + residual (act: a key of ACTS)."""
+        check(LIB.s3e_mul_mat_act(self.handle, w.handle, X.ptr, M, _ptr(bias), ACTS[act], _ptr(residual), Y.ptr, _ptr(ws),
+                                  ws.nbytes if ws else 0), "s3e_mul_mat_act")
 
     def kv_write(self, cache: KVCache, ggml_type: int, k: DeviceBuffer, k_nb, v: DeviceBuffer, v_nb,
                  slots: DeviceBuffer, n: int):

@@ -34,16 +34,23 @@ typedef uint32_t kv_u4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ kv_h2 as_h2(uint32_t x) { return __builtin_bit_cast(kv_h2, x); }
 
+// (x & mask) | magic as one v_and_or_b32: with both constants literal the
+// compiler makes two instructions of it, so they are kept in registers.
+struct KvMagic {
+    uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, e = 0x64006400u;
+    __device__ __forceinline__ KvMagic() { __asm__("" : "+v"(lo), "+v"(hi), "+v"(e)); }
+};
+
 // The eight codes of a word as fp16, exactly.  A code's bits below the exponent
 // of 1024 are 1024 + code (of 64 after the scale, for the nibbles four bits up).
-__device__ __forceinline__ kv_h8 word_h8_q4(uint32_t x) {
+__device__ __forceinline__ kv_h8 word_h8_q4(uint32_t x, const KvMagic &M) {
     const uint32_t y = x >> 8;
     const kv_h2 k = {(_Float16)1032.f, (_Float16)1032.f}, k16 = {(_Float16)-72.f, (_Float16)-72.f},
                 s16 = {(_Float16)0.0625f, (_Float16)0.0625f};
-    const kv_h2 a = as_h2((x & 0x000f000fu) | 0x64006400u) - k;
-    const kv_h2 b = __builtin_elementwise_fma(as_h2((x & 0x00f000f0u) | 0x64006400u), s16, k16);
-    const kv_h2 c = as_h2((y & 0x000f000fu) | 0x64006400u) - k;
-    const kv_h2 d = __builtin_elementwise_fma(as_h2((y & 0x00f000f0u) | 0x64006400u), s16, k16);
+    const kv_h2 a = as_h2((x & M.lo) | M.e) - k;
+    const kv_h2 b = __builtin_elementwise_fma(as_h2((x & M.hi) | M.e), s16, k16);
+    const kv_h2 c = as_h2((y & M.lo) | M.e) - k;
+    const kv_h2 d = __builtin_elementwise_fma(as_h2((y & M.hi) | M.e), s16, k16);
     return kv_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 __device__ __forceinline__ kv_h8 word_h8_q8(uint32_t x, uint32_t y) {
@@ -84,8 +91,8 @@ struct KvHalf {
             d[b] = __builtin_bit_cast(kv_h8, kv_u4{x.x, x.y, x.z, x.w});
         }
     }
-    __device__ __forceinline__ kv_h8 word(int i) const {
-        if constexpr (Q == 4) return word_h8_q4(w[i]);
+    __device__ __forceinline__ kv_h8 word(int i, const KvMagic &M) const {
+        if constexpr (Q == 4) return word_h8_q4(w[i], M);
         else return word_h8_q8(w[2 * i], w[2 * i + 1]);
     }
 };
@@ -99,12 +106,32 @@ __device__ __forceinline__ float sum_over_keys(float x) {
     return x + __shfl_xor(x, 32, 64);
 }
 
+// Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
+// through an accumulation register; more where the registers suffice.
+constexpr int kv_waves(int Q, int NB, bool F32, int NT) {
+    if (NT > 1 || NB == 8) return 2;
+    return NB <= 2 ? 4 : 3;
+}
+
+// P·d of two neighbouring keys as an fp16 pair, each product rounded once.
+__device__ __forceinline__ uint32_t scaled_pair(float p0, float p1, uint32_t d) {
+    uint32_t r;
+    __asm__("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,1,0]\n\tv_fma_mixhi_f16 %0, %2, %3, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
+            : "=&v"(r) : "v"(p0), "v"(p1), "v"(d));
+    return r;
+}
+
+// A mask over the fp16 pair of keys 2j, 2j + 1: zeros for those in `hidden`.
+__device__ __forceinline__ uint32_t keep_pair(uint32_t hidden, int j) {
+    return (hidden >> 2 * j & 1 ? 0u : 0xffffu) | (hidden >> 2 * j & 2 ? 0u : 0xffff0000u);
+}
+
 // One work-group: NT · 16 columns of a sequence and key/value head against one
 // range of its keys; its four waves take chunks in turn and are joined in LDS.
 // A chunk's K words for the wave's next turn are loaded as soon as the scores
 // are done with these, its V words behind the second product.
 template <int Q, int NB, bool F32, int NT>
-__global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
+__global__ __launch_bounds__(256, kv_waves(Q, NB, F32, NT)) void k_kv_attn(KvAttnArgs a) {
     using C = KvChunk<Q, NB>;
     constexpr int D = 32 * NB, W = 2 * NB;  // W: 16-channel tiles of V
     constexpr int PARTS = F32 ? 2 : 1;      // fp16 operands of an fp32 value
@@ -198,6 +225,7 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
                 for (int j = 0; j < 8; j++) {
                     float x = __builtin_amdgcn_ldexpf(v[b][j], -e);
                     if (a.neg) x = -x;
+                    __asm__("" : "+v"(x));  // one value for hi and for lo
                     const _Float16 hi = (_Float16)x;
                     qf[n][b][0][j] = hi;
                     qf[n][b][PARTS - 1][j] = (_Float16)(x - (float)hi);
@@ -216,6 +244,7 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
     }
     int ed = -24;  // |scales of V so far| ≤ 2^ed
 
+    const KvMagic M;
     const int gsh = a.c.page_shift - 5;
     const int64_t cpp = 1 << gsh;  // chunks of a page and head
     const int32_t *pages = a.pages + s * a.pages_ld;
@@ -247,26 +276,39 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
             bool have_n = have;
             const uint8_t *pn = place(more ? gn : g, have_n);
 
-            // ---- Sᵀ = K·Qᵀ, times K's scales
+            // ---- Sᵀ = K·Qᵀ, times K's scales: a block's sums are scaled behind
+            // the next block's MFMAs.  (The scheduling barriers keep the
+            // compiler from converting every word, or loading the next chunk's,
+            // before the first MFMA: it would spill.)
             float t[NT][8];
+            kv_f4 m[2][NT][2];
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int b = 0; b <= NB; b++) {
+                if (b < NB) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) t[n][j] = 0.f;
+                    for (int h = 0; h < 2; h++) {
+                        const kv_h8 kw = K.word(h * NB + b, M);
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+                        for (int n = 0; n < NT; n++) {
+                            kv_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const kv_h8 kw = K.word(h * NB + b);
-#pragma unroll
-                    for (int n = 0; n < NT; n++) {
-                        kv_f4 m = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int x = PARTS - 1; x >= 0; x--) m = __builtin_amdgcn_mfma_f32_16x16x32_f16(kw, qf[n][b][x], m, 0, 0, 0);
-#pragma unroll
-                        for (int i = 0; i < 4; i++) t[n][4 * h + i] = __builtin_fmaf((float)K.d[b][4 * h + i], m[i], t[n][4 * h + i]);
+                            for (int i = PARTS - 1; i >= 0; i--) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kw, qf[n][b][i], x, 0, 0, 0);
+                            m[b & 1][n][h] = x;
+                        }
                     }
                 }
+                if (b > 0) {
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const float x = m[(b - 1) & 1][n][j >> 2][j & 3], d = (float)K.d[b - 1][j];
+                            t[n][j] = b == 1 ? d * x : __builtin_fmaf(d, x, t[n][j]);
+                            __asm__ volatile("" : "+v"(t[n][j]));  // (here, not behind the next branch with every block's sums held)
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (more) K.load(pn, lane);
 
             // ---- scores, in powers of two; masked ones −∞
@@ -277,6 +319,7 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
 #pragma unroll
                 for (int j = 0; j < 8; j++) t[n][j] *= cs[n];
             uint32_t hidden[NT];  // bit j: key key0 + j is masked
+            bool partly = false;  // a scale that is no number, at a key that some columns see and others do not
             if (special) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
@@ -301,6 +344,23 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
                         hidden[n] |= t[n][j] == -INFINITY ? 1u << j : 0u;
                     }
                 }
+                // a masked key's probability is zero, but V's scale there may be
+                // no number: zero where none of this lane's columns sees the key
+                uint32_t all = hidden[0], any = hidden[0];
+#pragma unroll
+                for (int n = 1; n < NT; n++) all &= hidden[n], any |= hidden[n];
+                uint32_t odd = 0;  // keys some column sees, with a scale that is no number
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    kv_u4 d = __builtin_bit_cast(kv_u4, V.d[b]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        d[j] &= keep_pair(all, j);
+                        odd |= ((d[j] & 0x7c00u) == 0x7c00u ? 1u << 2 * j : 0u) | ((d[j] & 0x7c000000u) == 0x7c000000u ? 2u << 2 * j : 0u);
+                    }
+                    V.d[b] = __builtin_bit_cast(kv_h8, d);
+                }
+                if constexpr (NT > 1) partly = __builtin_amdgcn_ballot_w64(odd & any) != 0;
             }
 
             // ---- the references, where a score or a scale outgrew them
@@ -361,25 +421,43 @@ __global__ __launch_bounds__(256) void k_kv_attn(KvAttnArgs a) {
             // ---- Oᵀ += Vᵀ·(P·d)ᵀ, block by block of V's channels
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                kv_h8 p[NT][PARTS];
+                kv_u4 p[NT][PARTS];
+                const kv_u4 d = __builtin_bit_cast(kv_u4, V.d[b]);
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        float x = t[n][j] * (float)V.d[b][j];
-                        if (special && (hidden[n] >> j & 1)) x = 0.f;  // whatever the masked key's scale is
-                        const _Float16 hi = (_Float16)x;
-                        p[n][0][j] = hi;
-                        if constexpr (F32) p[n][PARTS - 1][j] = (_Float16)(x - (float)hi);
+                    for (int j = 0; j < 4; j++) {
+                        if constexpr (!F32) {
+                            p[n][0][j] = scaled_pair(t[n][2 * j], t[n][2 * j + 1], d[j]);
+                        } else {
+                            const kv_h2 dd = as_h2(d[j]);
+                            float x = t[n][2 * j] * (float)dd[0], y = t[n][2 * j + 1] * (float)dd[1];
+                            // one value for hi and for lo: folded into a mixed fma, hi alone would be rounded from the exact product
+                            __asm__("" : "+v"(x), "+v"(y));
+                            const kv_h2 hi = {(_Float16)x, (_Float16)y};
+                            p[n][0][j] = __builtin_bit_cast(uint32_t, hi);
+                            p[n][PARTS - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
+                        }
                     }
-#pragma unroll
-                for (int w = 2 * b; w < 2 * b + 2; w++) {
-                    const kv_h8 vw = V.word(w);
+                if (NT > 1 && partly) {
+                    __asm__ volatile("");  // (a branch, not selects)
 #pragma unroll
                     for (int n = 0; n < NT; n++)
 #pragma unroll
-                        for (int x = 0; x < PARTS; x++) acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw, p[n][x], acc[n][w], 0, 0, 0);
+                        for (int x = 0; x < PARTS; x++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) p[n][x][j] &= keep_pair(hidden[n], j);
                 }
+#pragma unroll
+                for (int w = 2 * b; w < 2 * b + 2; w++) {
+                    const kv_h8 vw = V.word(w, M);
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int x = 0; x < PARTS; x++)
+                            acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw, __builtin_bit_cast(kv_h8, p[n][x]), acc[n][w], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
             if (!more) break;
             V.load(pn + C::HALF, lane);

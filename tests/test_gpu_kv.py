@@ -315,6 +315,13 @@ def test_attention(ctx, t, io, heads, nh, D, page, lens, more):
     Batch(ctx, t, io, heads, nh, D, page, lens, seed=nh * D + len(lens), **more).check()
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_pairs_are_whole(ctx, t):
+    # the high half of every fp32 pair is the one its low half completes: 40 x 10^4 products a call, ties among them
+    for seed in range(6):
+        Batch(ctx, t, s3e.TYPE_F32, 2, 4, 64, 32, [(45, 45), (7, 7)], seed=seed).check()
+
+
 @pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
 def test_attention_writes_in_place(ctx, io):
     x = Batch(ctx, ref.Q4_0, io, 2, 4, 64, 64, [(5, 700), (2, 90)], seed=4)

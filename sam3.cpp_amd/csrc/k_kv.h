@@ -76,13 +76,15 @@ struct KvAttnArgs {
     int64_t mask_ld = 0;
     int mask_vec = 0;
     void *o = nullptr;
-    float scale = 0.f;      // |scale| · log2(e)
-    int neg = 0;            // scale < 0
+    float scale = 0.f;      // |scale| · log2(e), of a zero scale 1
+    int sign = 1;           // the scale's: −1, 0 or 1
     int causal = 0;
     int n_seq = 0, n_tokens = 0, max_q = 0, nh = 0;
     int64_t max_kv = 0;
-    int nt = 1;             // column tiles of 16 a work-group
+    int tile = 0;           // the kernel for many columns
+    int nt = 1;             // column tiles of 16 a wave
     int ctiles = 1;         // work-groups over the columns of a sequence and head
+    int goal = 0;           // work-groups to aim at with the split over keys
     // keys a work-group takes (a multiple of 128) and the number of such
     // ranges; nsplit > 1: unnormalised outputs to part_o [nsplit][tokens][nh][D]
     // and (reference, sum) to part_ml [nsplit][tokens][nh][2]
@@ -93,8 +95,9 @@ struct KvAttnArgs {
 hipError_t launch_kv_attn_q4(const KvAttnArgs &a, bool f32, hipStream_t st);
 hipError_t launch_kv_attn_q8(const KvAttnArgs &a, bool f32, hipStream_t st);
 hipError_t launch_kv_combine(const KvAttnArgs &a, bool f32, hipStream_t st);
-// Column tiles a work-group takes where a sequence and head have `cols` columns.
-int kv_attn_nt(int type, int D, bool f32, int64_t cols);
+// The kernel, column tiles and work-groups over the columns where a sequence and
+// head have `cols` of them.
+void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols);
 
 // The reference exponent of a column that has seen no key.
 constexpr float KV_NONE = -3.0e38f;

@@ -331,55 +331,65 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
     }
 }
 
-// The output row of one query and head from its key ranges: each range's
-// unnormalised output and sum are in units of 2^reference.  A work-group takes
-// one row; D/4 threads hold it and the others take further ranges, joined in
-// LDS in a fixed order.
-template <int D, bool F32>
+// Output rows (query, head) from their key ranges: each range's unnormalised
+// output and sum are in units of 2^reference.  D/4 threads hold a row.  Where a
+// row has many ranges a work-group takes one row (SPREAD), its other threads
+// further ranges, joined in LDS in a fixed order; where it has few, a row each.
+template <int D, bool F32, bool SPREAD>
 __global__ __launch_bounds__(256) void k_kv_combine(KvAttnArgs a) {
     constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-    __shared__ float4 acc_lds[GROUPS][LANES];
-    __shared__ float sum_lds[GROUPS], top_lds[4];
+    __shared__ float4 acc_lds[SPREAD ? GROUPS : 1][LANES];
+    __shared__ float sum_lds[GROUPS];
     const int tid = threadIdx.x, s = blockIdx.y;
     const int q0 = min(max(a.q_start[s], 0), a.n_tokens), q1 = min(max(a.q_start[s + 1], q0), a.n_tokens);
-    const int i = blockIdx.x / a.nh, h = blockIdx.x - i * a.nh;
-    if (i >= min(q1 - q0, a.max_q)) return;
+    const int gr = tid / LANES, d4 = tid % LANES;
+    const int r = SPREAD ? blockIdx.x : blockIdx.x * GROUPS + gr;
+    const int i = r / a.nh, h = r - i * a.nh;
+    // (of a spread row all threads leave or none; GROUPS · LANES may be less than 256)
+    if (i >= min(q1 - q0, a.max_q) || (!SPREAD && gr >= GROUPS)) return;
     const int64_t len = min((int64_t)max(a.kv_len[s], 0), a.max_kv);
     const int n = (int)min((len + a.chunk - 1) / a.chunk, (int64_t)a.nsplit);
     const int64_t row = (int64_t)(q0 + i) * a.nh + h, rows = (int64_t)a.n_tokens * a.nh;
+    const float2 *ml = (const float2 *)a.part_ml + row;
+    const float *po = a.part_o + row * D + 4 * d4;
+    // a range without a key for this row holds zeros at KV_NONE
     float top = KV_NONE;
-    for (int k = tid; k < n; k += 256) top = fmaxf(top, a.part_ml[(k * rows + row) * 2]);
+    if constexpr (SPREAD) {
+        for (int k = tid & 63; k < n; k += 64) top = fmaxf(top, ml[k * rows].x);
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-    if ((tid & 63) == 0) top_lds[tid >> 6] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(top_lds[0], top_lds[1]), fmaxf(top_lds[2], top_lds[3]));
-    const int gr = tid / LANES, d4 = tid % LANES;
+        for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+    } else {
+#pragma unroll 4
+        for (int k = 0; k < n; k++) top = fmaxf(top, ml[k * rows].x);
+    }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
     if (gr < GROUPS) {
 #pragma unroll 4
-        for (int k = gr; k < n; k += GROUPS) {
-            const float2 ml = *(const float2 *)(a.part_ml + (k * rows + row) * 2);
-            const float4 o = *(const float4 *)(a.part_o + (k * rows + row) * D + 4 * d4);
-            // a range without a key for this row holds zeros at KV_NONE
-            const float w = ml.x == KV_NONE ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+        for (int k = SPREAD ? gr : 0; k < n; k += SPREAD ? GROUPS : 1) {
+            const float2 m = ml[k * rows];
+            const float4 o = *(const float4 *)(po + k * rows * D);
+            const float w = m.x == KV_NONE ? 0.f : __builtin_amdgcn_exp2f(m.x - top);
             acc.x = __builtin_fmaf(w, o.x, acc.x);
             acc.y = __builtin_fmaf(w, o.y, acc.y);
             acc.z = __builtin_fmaf(w, o.z, acc.z);
             acc.w = __builtin_fmaf(w, o.w, acc.w);
-            sum = __builtin_fmaf(w, ml.y, sum);
+            sum = __builtin_fmaf(w, m.y, sum);
         }
-        acc_lds[gr][d4] = acc;
-        if (d4 == 0) sum_lds[gr] = sum;
+        if constexpr (SPREAD) {
+            acc_lds[gr][d4] = acc;
+            if (d4 == 0) sum_lds[gr] = sum;
+        }
     }
-    __syncthreads();
-    if (gr != 0) return;
+    if constexpr (SPREAD) {
+        __syncthreads();
+        if (gr != 0) return;
 #pragma unroll
-    for (int k = 1; k < GROUPS; k++) {
-        const float4 o = acc_lds[k][d4];
-        acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
-        sum += sum_lds[k];
+        for (int k = 1; k < GROUPS; k++) {
+            const float4 o = acc_lds[k][d4];
+            acc.x += o.x, acc.y += o.y, acc.z += o.z, acc.w += o.w;
+            sum += sum_lds[k];
+        }
     }
     const float inv = sum == 0.f ? 0.f : 1.0f / sum;  // no key at all: zeros
     if constexpr (F32) {
@@ -430,18 +440,22 @@ hipError_t launch_kv_read(const KvReadArgs &a, bool f32, hipStream_t st) {
 }
 
 hipError_t launch_kv_combine(const KvAttnArgs &a, bool f32, hipStream_t st) {
-    const dim3 grid(a.max_q * a.nh, a.n_seq);
-    auto go = [&](auto d) {
-        if (f32) hipLaunchKernelGGL((k_kv_combine<d(), true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_kv_combine<d(), false>), grid, dim3(256), 0, st, a);
+    auto go = [&](auto d, auto f) {
+        constexpr int GROUPS = 256 / (d() / 4);
+        const int64_t rows = (int64_t)a.max_q * a.nh;
+        if (a.nsplit > 8)
+            hipLaunchKernelGGL((k_kv_combine<d(), f(), true>), dim3((unsigned)rows, a.n_seq), dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((k_kv_combine<d(), f(), false>), dim3((unsigned)((rows + GROUPS - 1) / GROUPS), a.n_seq), dim3(256), 0, st, a);
         return hipGetLastError();
     };
+    auto by = [&](auto d) { return f32 ? go(d, std::true_type{}) : go(d, std::false_type{}); };
     switch (a.c.D) {
-        case 32: return go(std::integral_constant<int, 32>{});
-        case 64: return go(std::integral_constant<int, 64>{});
-        case 96: return go(std::integral_constant<int, 96>{});
-        case 128: return go(std::integral_constant<int, 128>{});
-        case 256: return go(std::integral_constant<int, 256>{});
+        case 32: return by(std::integral_constant<int, 32>{});
+        case 64: return by(std::integral_constant<int, 64>{});
+        case 96: return by(std::integral_constant<int, 96>{});
+        case 128: return by(std::integral_constant<int, 128>{});
+        case 256: return by(std::integral_constant<int, 256>{});
         default: return hipErrorInvalidValue;
     }
 }

@@ -65,30 +65,27 @@ __device__ __forceinline__ kv_h8 word_h8_q8(uint32_t x, uint32_t y) {
     return kv_h8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// K's or V's half of a chunk as one wave holds it: its words, and the scales
-// of keys 8a .. 8a + 8 of each block.
+// K's or V's half of a chunk in LDS, as a wave's lanes read it: their words, and
+// the scales of keys 8a .. 8a + 8 of each block.
+typedef __attribute__((address_space(3))) const uint8_t *kv_lds;
+__device__ __forceinline__ kv_u4 lds16(kv_lds p) { return *(__attribute__((address_space(3))) const kv_u4 *)p; }
+__device__ __forceinline__ uint64_t lds8(kv_lds p) { return *(__attribute__((address_space(3))) const uint64_t *)p; }
 template <int Q, int NB>
 struct KvHalf {
     using C = KvChunk<Q, NB>;
     uint32_t w[C::WORDS * Q / 4];
-    kv_h8 d[NB];
-    __device__ __forceinline__ void load(const uint8_t *p, int lane) {
+    __device__ __forceinline__ void load(kv_lds p, int lane) {
 #pragma unroll
         for (int i = 0; i < C::PIECES; i++) {
-            const uint8_t *q = p + i * 1024 + lane * (C::width(i) * Q);
+            const kv_lds q = p + i * 1024 + lane * (C::width(i) * Q);
             const int n = C::width(i) * Q / 4, at = i * 4;
             if (n == 4) {
-                const uint4 x = gload16(q);
-                w[at] = x.x, w[at + 1] = x.y, w[at + 2] = x.z, w[at + 3] = x.w;
+                const kv_u4 x = lds16(q);
+                w[at] = x[0], w[at + 1] = x[1], w[at + 2] = x[2], w[at + 3] = x[3];
             } else {
-                const uint2 x = gload8(q);
-                w[at] = x.x, w[at + 1] = x.y;
+                const uint64_t x = lds8(q);
+                w[at] = (uint32_t)x, w[at + 1] = (uint32_t)(x >> 32);
             }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            const uint4 x = gload16(p + C::CODES + b * 64 + (lane >> 4) * 16);
-            d[b] = __builtin_bit_cast(kv_h8, kv_u4{x.x, x.y, x.z, x.w});
         }
     }
     __device__ __forceinline__ kv_h8 word(int i, const KvMagic &M) const {
@@ -96,6 +93,9 @@ struct KvHalf {
         else return word_h8_q8(w[2 * i], w[2 * i + 1]);
     }
 };
+// The scales of block b for the keys of a lane group.
+template <int Q, int NB>
+__device__ __forceinline__ kv_u4 scales_of(kv_lds half, int b, int ka) { return lds16(half + KvChunk<Q, NB>::CODES + b * 64 + ka * 16); }
 
 __device__ __forceinline__ float max_over_keys(float x) {
     x = fmaxf(x, __shfl_xor(x, 16, 64));
@@ -104,13 +104,6 @@ __device__ __forceinline__ float max_over_keys(float x) {
 __device__ __forceinline__ float sum_over_keys(float x) {
     x += __shfl_xor(x, 16, 64);
     return x + __shfl_xor(x, 32, 64);
-}
-
-// Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
-// through an accumulation register; more where the registers suffice.
-constexpr int kv_waves(int Q, int NB, bool F32, int NT) {
-    if (NT > 1 || NB == 8) return 2;
-    return NB <= 2 ? 4 : 3;
 }
 
 // P·d of two neighbouring keys as an fp16 pair, each product rounded once.
@@ -126,425 +119,650 @@ __device__ __forceinline__ uint32_t keep_pair(uint32_t hidden, int j) {
     return (hidden >> 2 * j & 1 ? 0u : 0xffffu) | (hidden >> 2 * j & 2 ? 0u : 0xffff0000u);
 }
 
-// One work-group: NT · 16 columns of a sequence and key/value head against one
-// range of its keys; its four waves take chunks in turn and are joined in LDS.
-// A chunk's K words for the wave's next turn are loaded as soon as the scores
-// are done with these, its V words behind the second product.
-template <int Q, int NB, bool F32, int NT>
-__global__ __launch_bounds__(256, kv_waves(Q, NB, F32, NT)) void k_kv_attn(KvAttnArgs a) {
-    using C = KvChunk<Q, NB>;
-    constexpr int D = 32 * NB, W = 2 * NB;  // W: 16-channel tiles of V
-    constexpr int PARTS = F32 ? 2 : 1;      // fp16 operands of an fp32 value
-    __shared__ kv_f4 lds[2][NT * W][64];
-    __shared__ float lds_ml[2][NT][2][64];
+// s_waitcnt's field for at most n vector-memory operations under way.
+constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
-    const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, ka = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // work-group → (sequence, head, key range), column tile: those that read the
-    // same keys on one XCD, and the later (under a causal mask longer) tiles first
-    const int units = a.n_seq * a.c.heads * a.nsplit;
+// What a work-group is to do: its sequence, key/value head, key range and
+// first column; `some` where there is anything.
+struct KvTask {
+    bool some;
+    int split, kvh, q0, nq, ncols, len, c0, G;
+    int k_begin, k_end;  // of the tile: keys some of its columns see
+};
+template <int COLS>
+__device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
+    // work-group → (sequence, head, key range) unit and column tile: an XCD (every
+    // eighth work-group) takes a contiguous eighth of them, unit by unit, so that
+    // the tiles that read the same keys share its L2; whole units tile by tile,
+    // the later (under a causal mask longer) ones of every unit first, so that the
+    // short ones fill the gaps
+    KvTask t;
+    t.some = false;
+    const int units = a.n_seq * a.c.heads * a.nsplit, total = units * a.ctiles, per = (total + 7) >> 3;
+    const int i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per + i;
+    if (i >= per || at >= total) return t;
     int unit, ct;
-    {
-        const int id = blockIdx.x;
-        if (units >= 8) {
-            const int i = id >> 3;
-            unit = (i / a.ctiles) * 8 + (id & 7);
-            ct = a.ctiles - 1 - i % a.ctiles;
-        } else {
-            unit = id % units;
-            ct = a.ctiles - 1 - id / units;
-        }
+    if (units % 8 == 0) {
+        const int u = units >> 3;
+        unit = (i % u) * 8 + (blockIdx.x & 7);  // (dealt out: a long sequence's heads to every XCD)
+        ct = a.ctiles - 1 - i / u;
+    } else {
+        unit = at / a.ctiles;
+        ct = a.ctiles - 1 - at % a.ctiles;
     }
-    if (unit >= units) return;
-    const int split = unit % a.nsplit, sh = unit / a.nsplit;
-    const int s = sh / a.c.heads, kvh = sh - s * a.c.heads;
-    const int G = a.nh / a.c.heads;
-    const int q0 = min(max(a.q_start[s], 0), a.n_tokens), q1 = min(max(a.q_start[s + 1], q0), a.n_tokens);
-    const int nq = q1 - q0, ncols = min(nq, a.max_q) * G, c0 = ct * (16 * NT);
-    if (c0 >= ncols) return;
-    const int len = (int)min((int64_t)max(a.kv_len[s], 0), a.max_kv);
-    // the keys that some column of the tile sees, and those that all of them see
-    const int i_first = c0 / G, i_last = (min(c0 + 16 * NT, ncols) - 1) / G;
-    const int see_all = a.causal ? min(len, len - nq + i_first + 1) : len;
-    const int see_any = a.causal ? min(len, len - nq + i_last + 1) : len;
-    const int64_t kb = split * a.chunk;
-    if (kb >= len && split > 0) return;  // past the sequence: no range the joining pass reads
-    const int k_begin = (int)kb, k_end = (int)min((int64_t)see_any, kb + a.chunk);
+    const int sh = unit / a.nsplit;
+    t.split = unit % a.nsplit;
+    s = sh / a.c.heads;
+    t.kvh = sh - s * a.c.heads;
+    t.G = a.nh / a.c.heads;
+    t.q0 = min(max(a.q_start[s], 0), a.n_tokens);
+    t.nq = min(max(a.q_start[s + 1], t.q0), a.n_tokens) - t.q0;
+    t.ncols = min(t.nq, a.max_q) * t.G;
+    t.c0 = ct * COLS;
+    if (t.c0 >= t.ncols) return t;
+    t.len = (int)min((int64_t)max(a.kv_len[s], 0), a.max_kv);
+    const int64_t kb = t.split * a.chunk;
+    if (kb >= t.len && t.split > 0) return t;  // past the sequence: no range the joining pass reads
+    const int i_last = (min(t.c0 + COLS, t.ncols) - 1) / t.G;
+    t.k_begin = (int)kb;
+    t.k_end = (int)min((int64_t)(a.causal ? min(t.len, t.len - t.nq + i_last + 1) : t.len), kb + a.chunk);
+    t.some = true;
+    return t;
+}
 
-    // this lane's column of each tile: its query, head and limit (past the
-    // last column: the last one's again, not stored)
+// Where a sequence's chunks lie.
+struct KvPlaces {
+    // (read by scalar loads: a vector load would wait behind every chunk under way)
+    typedef __attribute__((address_space(4))) const int32_t c_i32;
+    const c_i32 *pages;
+    const uint8_t *base;     // of this head in page 0
+    int64_t stride;          // bytes from page to page
+    int n_pages, gsh, bytes;
+    __device__ __forceinline__ KvPlaces(const KvAttnArgs &a, int s, int kvh, int bytes_)
+        : pages((c_i32 *)(a.pages + s * a.pages_ld)), n_pages((int)(a.c.slots >> a.c.page_shift)), gsh(a.c.page_shift - 5), bytes(bytes_) {
+        base = a.c.data + ((int64_t)kvh << gsh) * bytes;
+        stride = ((int64_t)a.c.heads << gsh) * bytes;
+    }
+    // chunk g; a page that the cache does not have is read as page 0 and masked
+    __device__ __forceinline__ const uint8_t *at(int g, bool &have) const {
+        const int p = pages[g >> gsh];
+        have = (unsigned)p < (unsigned)n_pages;
+        return base + (have ? p : 0) * stride + (g & ((1 << gsh) - 1)) * bytes;
+    }
+};
+
+// NT · 16 columns of one wave: queries, running sums and output.
+template <int NB, bool F32, int NT, bool FENCE>
+struct KvColumns {
+    static constexpr int D = 32 * NB, W = 2 * NB;  // W: 16-channel tiles of V
+    static constexpr int PARTS = F32 ? 2 : 1;      // fp16 operands of an fp32 value
+    static constexpr int VD = (NB * 16 + 63) / 64;
+
+    int c0, see_all;
     int lim[NT], tok[NT], head[NT];
-    float cs[NT];
+    float cs[NT];            // a score's units of log2
     kv_h8 qf[NT][NB][PARTS];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int c = c0 + 16 * n + col, i = min(c, ncols - 1) / G;
-        tok[n] = q0 + i;
-        head[n] = kvh * G + (min(c, ncols - 1) - i * G);
-        lim[n] = a.causal ? min(len, len - nq + i + 1) : len;
-        cs[n] = a.scale;
-        const int64_t at = tok[n] * a.q_st + head[n] * a.q_sh + 8 * ka;
-        if constexpr (!F32) {
-            const _Float16 *q = (const _Float16 *)a.q + at;
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                kv_h8 x;
-                if (a.q_vec) {
-                    x = *(const kv_h8 *)(q + 32 * b);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) x[j] = q[32 * b + j];
-                }
-                qf[n][b][0] = a.neg ? -x : x;
-            }
-        } else {
-            const float *q = (const float *)a.q + at;
-            float v[NB][8], top = 0.f;
-#pragma unroll
-            for (int b = 0; b < NB; b++) {
-                if (a.q_vec) {
-                    const float4 x = *(const float4 *)(q + 32 * b), y = *(const float4 *)(q + 32 * b + 4);
-                    v[b][0] = x.x, v[b][1] = x.y, v[b][2] = x.z, v[b][3] = x.w;
-                    v[b][4] = y.x, v[b][5] = y.y, v[b][6] = y.z, v[b][7] = y.w;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[b][j] = q[32 * b + j];
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[b][j]));
-            }
-            top = max_over_keys(top);
-            // q = 2^e · (hi + lo), the row's largest in [2^14, 2^15): hi + lo is
-            // 22 bits of each value down to 2^-14 of that, 2^-39 of it below
-            int e = 0;
-            if (top > 0.f && top < INFINITY) e = __builtin_amdgcn_frexp_expf(top) - 15;
-            cs[n] = __builtin_amdgcn_ldexpf(a.scale, e);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float x = __builtin_amdgcn_ldexpf(v[b][j], -e);
-                    if (a.neg) x = -x;
-                    __asm__("" : "+v"(x));  // one value for hi and for lo
-                    const _Float16 hi = (_Float16)x;
-                    qf[n][b][0][j] = hi;
-                    qf[n][b][PARTS - 1][j] = (_Float16)(x - (float)hi);
-                }
-        }
-    }
-
     kv_f4 acc[NT][W];
     float ref[NT], sum[NT];  // reference (log2) and this lane's part of the sum
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        ref[n] = KV_NONE;
-        sum[n] = 0.f;
-#pragma unroll
-        for (int w = 0; w < W; w++) acc[n][w] = kv_f4{0.f, 0.f, 0.f, 0.f};
-    }
-    int ed = -24;  // |scales of V so far| ≤ 2^ed
-
+    int ed;                  // |scales of V so far| ≤ 2^ed
     const KvMagic M;
-    const int gsh = a.c.page_shift - 5;
-    const int64_t cpp = 1 << gsh;  // chunks of a page and head
-    const int32_t *pages = a.pages + s * a.pages_ld;
-    const int64_t n_pages = a.c.slots >> a.c.page_shift;
-    // a page that the cache does not have is read as page 0 and masked
-    auto place = [&](int g, bool &have) -> const uint8_t * {
-        const int64_t p = pages[g >> gsh];
-        have = p >= 0 && p < n_pages;
-        return a.c.data + (((have ? p : 0) * a.c.heads + kvh) * cpp + (g & (cpp - 1))) * C::BYTES;
-    };
 
-    const int g_end = (k_end + 31) >> 5;
-    int g = (k_begin >> 5) + wave;
-    KvHalf<Q, NB> K, V;
-    // V's scales once more, a dword a lane (each of the chunk's NB · 16 is some lane's)
-    constexpr int VD = (NB * 16 + 63) / 64;
-    uint32_t vds[VD];
-    bool have = true;
-    if (k_begin < k_end && g < g_end) {
-        const uint8_t *p = place(g, have);
-        K.load(p, lane);
-        V.load(p + C::HALF, lane);
+    // This lane's column of each tile: its query, head and limit (past the last
+    // column: the last one's again, not stored).
+    __device__ __forceinline__ void start(const KvAttnArgs &a, const KvTask &k, int first, int lane) {
+        const int col = lane & 15, ka = lane >> 4;
+        c0 = first;
+        const int i_first = min(c0, k.ncols - 1) / k.G;
+        see_all = a.causal ? min(k.len, k.len - k.nq + i_first + 1) : k.len;
+        ed = -24;
 #pragma unroll
-        for (int i = 0; i < VD; i++)
-            vds[i] = *(const uint32_t *)(p + C::HALF + C::CODES + ((lane + 64 * i) % (NB * 16)) * 4);
-        while (true) {
-            const int gn = g + 4;
-            const bool more = gn < g_end;
-            bool have_n = have;
-            const uint8_t *pn = place(more ? gn : g, have_n);
-
-            // ---- Sᵀ = K·Qᵀ, times K's scales: a block's sums are scaled behind
-            // the next block's MFMAs.  (The scheduling barriers keep the
-            // compiler from converting every word, or loading the next chunk's,
-            // before the first MFMA: it would spill.)
-            float t[NT][8];
-            kv_f4 m[2][NT][2];
+        for (int n = 0; n < NT; n++) {
+            ref[n] = KV_NONE;
+            sum[n] = 0.f;
 #pragma unroll
-            for (int b = 0; b <= NB; b++) {
-                if (b < NB) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const kv_h8 kw = K.word(h * NB + b, M);
-#pragma unroll
-                        for (int n = 0; n < NT; n++) {
-                            kv_f4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                            for (int i = PARTS - 1; i >= 0; i--) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kw, qf[n][b][i], x, 0, 0, 0);
-                            m[b & 1][n][h] = x;
-                        }
-                    }
-                }
-                if (b > 0) {
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            const float x = m[(b - 1) & 1][n][j >> 2][j & 3], d = (float)K.d[b - 1][j];
-                            t[n][j] = b == 1 ? d * x : __builtin_fmaf(d, x, t[n][j]);
-                            __asm__ volatile("" : "+v"(t[n][j]));  // (here, not behind the next branch with every block's sums held)
-                        }
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (more) K.load(pn, lane);
-
-            // ---- scores, in powers of two; masked ones −∞
-            const int key0 = 32 * g + 8 * ka;
-            const bool special = a.mask || !have || 32 * g + 32 > see_all;
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) t[n][j] *= cs[n];
-            uint32_t hidden[NT];  // bit j: key key0 + j is masked
-            bool partly = false;  // a scale that is no number, at a key that some columns see and others do not
-            if (special) {
-#pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    if (a.mask) {
-                        const _Float16 *mp = a.mask + tok[n] * a.mask_ld + key0;
-                        float mv[8];
-                        if (a.mask_vec && key0 + 8 <= a.max_kv) {
-                            const kv_h8 x = *(const kv_h8 *)mp;
-#pragma unroll
-                            for (int j = 0; j < 8; j++) mv[j] = (float)x[j];
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) mv[j] = key0 + j < len ? (float)mp[j] : 0.f;
-                        }
-#pragma unroll
-                        for (int j = 0; j < 8; j++) t[n][j] = mv[j] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[j], 1.4426950408889634f, t[n][j]);
-                    }
-                    hidden[n] = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (!have || key0 + j >= lim[n]) t[n][j] = -INFINITY;
-                        hidden[n] |= t[n][j] == -INFINITY ? 1u << j : 0u;
-                    }
-                }
-                // a masked key's probability is zero, but V's scale there may be
-                // no number: zero where none of this lane's columns sees the key
-                uint32_t all = hidden[0], any = hidden[0];
-#pragma unroll
-                for (int n = 1; n < NT; n++) all &= hidden[n], any |= hidden[n];
-                uint32_t odd = 0;  // keys some column sees, with a scale that is no number
+            for (int w = 0; w < W; w++) acc[n][w] = kv_f4{0.f, 0.f, 0.f, 0.f};
+            const int c = min(c0 + 16 * n + col, k.ncols - 1), i = c / k.G;
+            tok[n] = k.q0 + i;
+            head[n] = k.kvh * k.G + (c - i * k.G);
+            lim[n] = a.causal ? min(k.len, k.len - k.nq + i + 1) : k.len;
+            const int64_t at = tok[n] * a.q_st + head[n] * a.q_sh + 8 * ka;
+            if constexpr (!F32) {
+                cs[n] = a.scale;
+                const _Float16 *q = (const _Float16 *)a.q + at;
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    kv_u4 d = __builtin_bit_cast(kv_u4, V.d[b]);
+                    kv_h8 x;
+                    if (a.q_vec) {
+                        x = *(const kv_h8 *)(q + 32 * b);
+                    } else {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        d[j] &= keep_pair(all, j);
-                        odd |= ((d[j] & 0x7c00u) == 0x7c00u ? 1u << 2 * j : 0u) | ((d[j] & 0x7c000000u) == 0x7c000000u ? 2u << 2 * j : 0u);
+                        for (int j = 0; j < 8; j++) x[j] = q[32 * b + j];
                     }
-                    V.d[b] = __builtin_bit_cast(kv_h8, d);
+                    qf[n][b][0] = a.sign < 0 ? -x : (a.sign == 0 ? x * (_Float16)0.f : x);
                 }
-                if constexpr (NT > 1) partly = __builtin_amdgcn_ballot_w64(odd & any) != 0;
+            } else {
+                const float *q = (const float *)a.q + at;
+                float v[NB][8], top = 0.f;
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if (a.q_vec) {
+                        const float4 x = *(const float4 *)(q + 32 * b), y = *(const float4 *)(q + 32 * b + 4);
+                        v[b][0] = x.x, v[b][1] = x.y, v[b][2] = x.z, v[b][3] = x.w;
+                        v[b][4] = y.x, v[b][5] = y.y, v[b][6] = y.z, v[b][7] = y.w;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) v[b][j] = q[32 * b + j];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(v[b][j]));
+                }
+                top = max_over_keys(top);
+                // q = 2^e · (hi + lo), the row's largest in [2^14, 2^15): hi + lo is
+                // 22 bits of each value down to 2^-14 of that, 2^-39 of it below
+                int e = 0;
+                if (top > 0.f && top < INFINITY) e = __builtin_amdgcn_frexp_expf(top) - 15;
+                // (neither zero nor infinite, which would make −∞ or 0 no number)
+                cs[n] = fminf(fmaxf(__builtin_amdgcn_ldexpf(a.scale, e), 1.17549435e-38f), 3.40282347e38f);
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        float x = __builtin_amdgcn_ldexpf(v[b][j], -e) * (float)a.sign;
+                        __asm__("" : "+v"(x));  // one value for hi and for lo
+                        const _Float16 hi = (_Float16)x;
+                        qf[n][b][0][j] = hi;
+                        qf[n][b][PARTS - 1][j] = (_Float16)(x - (float)hi);
+                    }
             }
+        }
+    }
 
-            // ---- the references, where a score or a scale outgrew them
-            bool grow = false;
+    // One chunk: keys 32g .. 32g + 32 (`have`: of a page the cache has).  The
+    // operands come by word: kword(i), vword(i) as fp16, kscale(b), vscale(b)
+    // the scales of this lane's eight keys, vbits(i) dwords of V's scales, of
+    // which each of the chunk's NB · 16 is some lane's.
+    template <typename KW, typename KS, typename VW, typename VS, typename VB>
+    __device__ __forceinline__ void chunk(const KvAttnArgs &a, int len, int g, bool have, int lane, KW kword, KS kscale, VW vword,
+                                          VS vscale, VB vbits) {
+        // ---- Sᵀ = K·Qᵀ, times K's scales: the next block's words are made
+        // between a block's MFMAs and their use.  (The scheduling barriers keep
+        // the compiler from making every word before the first MFMA: it would
+        // spill.)
+        float t[NT][8];
+        kv_h8 kw[2] = {kword(0), kword(NB)};
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                float mx = fmaxf(fmaxf(t[n][0], t[n][1]), t[n][2]);
-                mx = fmaxf(fmaxf(mx, t[n][3]), t[n][4]);
-                mx = fmaxf(fmaxf(mx, t[n][5]), fmaxf(t[n][6], t[n][7]));
-                grow = grow || mx > ref[n] + (float)(15 - ed);
-            }
-            const uint32_t bound = (uint32_t)(ed >= -14 ? (ed + 15) << 10 : 1 << (ed + 24));  // fp16 bits of 2^ed
+        for (int b = 0; b < NB; b++) {
+            kv_f4 m[NT][2];
 #pragma unroll
-            for (int i = 0; i < VD; i++) grow = grow || (vds[i] & 0x7fffu) > bound || ((vds[i] >> 16) & 0x7fffu) > bound;
-            if (__builtin_amdgcn_ballot_w64(grow)) {
-                // V's largest scale among keys of the sequence; not those that are no numbers
-                uint32_t dm = 0;
-#pragma unroll
-                for (int i = 0; i < VD; i++) {
-                    const int k2 = 32 * g + 2 * ((lane + 64 * i) & 15);
-                    const uint32_t lo = vds[i] & 0x7fffu, hi = (vds[i] >> 16) & 0x7fffu;
-                    if (have && k2 < len && lo < 0x7c00u) dm = max(dm, lo);
-                    if (have && k2 + 1 < len && hi < 0x7c00u) dm = max(dm, hi);
-                }
-#pragma unroll
-                for (int x = 1; x < 64; x *= 2) dm = max(dm, (uint32_t)__shfl_xor((int)dm, x, 64));
-                // 2^en ≥ every scale: one above the exponent, or of a subnormal its bit length − 24
-                const int en = dm >= 0x400u ? (int)(dm >> 10) - 14 : 8 - (dm ? __builtin_clz(dm) : 32);
-                const int ed_n = max(ed, __builtin_amdgcn_readfirstlane(en));
+            for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    float mx = fmaxf(fmaxf(t[n][0], t[n][1]), t[n][2]);
-                    mx = fmaxf(fmaxf(mx, t[n][3]), t[n][4]);
-                    mx = fmaxf(fmaxf(mx, t[n][5]), fmaxf(t[n][6], t[n][7]));
-                    mx = max_over_keys(mx);
-                    // the reference is the largest score + ed − 7
-                    const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (float)(ed - 7);
-                    const float top = fmaxf(best, mx);
-                    const float ref_n = top <= KV_NONE ? KV_NONE : top + (float)(ed_n - 7);
-                    const float alpha = ref_n == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - ref_n);
-                    ref[n] = ref_n;
-                    sum[n] *= alpha;
+                    kv_f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < W; w++) acc[n][w] *= alpha;
+                    for (int i = PARTS - 1; i >= 0; i--) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(kw[h], qf[n][b][i], x, 0, 0, 0);
+                    m[n][h] = x;
                 }
-                ed = ed_n;
-            }
-
-            // ---- probabilities, in units of the reference
+            const kv_h8 kd = __builtin_bit_cast(kv_h8, kscale(b));
+            if (b + 1 < NB) kw[0] = kword(b + 1), kw[1] = kword(NB + b + 1);
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    t[n][j] = __builtin_amdgcn_exp2f(t[n][j] - ref[n]);
-                    sum[n] += t[n][j];
+                    t[n][j] = __builtin_fmaf((float)kd[j], m[n][j >> 2][j & 3], b == 0 ? 0.f : t[n][j]);
+                    __asm__ volatile("" : "+v"(t[n][j]));  // (here, not behind the next branch with every block's sums held)
                 }
-
-            // ---- Oᵀ += Vᵀ·(P·d)ᵀ, block by block of V's channels
+            if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
+        }
+        uint32_t vds[VD];
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                kv_u4 p[NT][PARTS];
-                const kv_u4 d = __builtin_bit_cast(kv_u4, V.d[b]);
+        for (int i = 0; i < VD; i++) vds[i] = vbits(i);
+
+        // ---- masked scores −∞; with a mask the scores are in powers of two
+        const int key0 = 32 * g + 8 * (lane >> 4);
+        const bool special = a.mask || !have || 32 * g + 32 > see_all;
+        uint32_t hidden[NT], all = 0;  // bit j: key key0 + j is masked, in a column, in all of the lane's
+        bool partly = false;  // a scale that is no number, at a key that some columns see and others do not
+        if (special) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (a.mask) {
+                    const _Float16 *mp = a.mask + tok[n] * a.mask_ld + key0;
+                    float mv[8];
+                    if (a.mask_vec && key0 + 8 <= a.max_kv) {
+                        const kv_h8 x = *(const kv_h8 *)mp;
+#pragma unroll
+                        for (int j = 0; j < 8; j++) mv[j] = (float)x[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; j++) mv[j] = (float)mp[min(j, len - 1 - key0)];  // (all at once: past the end any value does)
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        t[n][j] = mv[j] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[j], 1.4426950408889634f, t[n][j] * cs[n]);
+                }
+                hidden[n] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (!have || key0 + j >= lim[n]) t[n][j] = -INFINITY;
+                    hidden[n] |= t[n][j] == -INFINITY ? 1u << j : 0u;
+                }
+            }
+            // a masked key's probability is zero, but V's scale there may be no
+            // number: zero below where none of this lane's columns sees the key
+            all = hidden[0];
+            uint32_t any = hidden[0];
+#pragma unroll
+            for (int n = 1; n < NT; n++) all &= hidden[n], any |= hidden[n];
+            if constexpr (NT > 1) {
+                uint32_t odd = 0;  // keys with a scale that is no number
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const kv_u4 d = vscale(b);
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        odd |= ((d[j] & 0x7c00u) == 0x7c00u ? 1u << 2 * j : 0u) | ((d[j] & 0x7c000000u) == 0x7c000000u ? 2u << 2 * j : 0u);
+                }
+                partly = __builtin_amdgcn_ballot_w64(odd & any & ~all) != 0;
+            }
+        }
+
+        // ---- the references, where a score or a scale outgrew them
+        float mx[NT], c1[NT];
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            c1[n] = a.mask ? 1.f : cs[n];
+            float x = fmaxf(fmaxf(t[n][0], t[n][1]), t[n][2]);
+            x = fmaxf(fmaxf(x, t[n][3]), t[n][4]);
+            mx[n] = fmaxf(fmaxf(x, t[n][5]), fmaxf(t[n][6], t[n][7])) * c1[n];
+            grow = grow || mx[n] > ref[n] + (float)(15 - ed);
+        }
+        const uint32_t bound = (uint32_t)(ed >= -14 ? (ed + 15) << 10 : 1 << (ed + 24));  // fp16 bits of 2^ed
+#pragma unroll
+        for (int i = 0; i < VD; i++) grow = grow || (vds[i] & 0x7fffu) > bound || ((vds[i] >> 16) & 0x7fffu) > bound;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+            // V's largest scale among keys of the sequence; not those that are no numbers
+            uint32_t dm = 0;
+#pragma unroll
+            for (int i = 0; i < VD; i++) {
+                const int k2 = 32 * g + 2 * ((lane + 64 * i) & 15);
+                const uint32_t lo = vds[i] & 0x7fffu, hi = (vds[i] >> 16) & 0x7fffu;
+                if (have && k2 < len && lo < 0x7c00u) dm = max(dm, lo);
+                if (have && k2 + 1 < len && hi < 0x7c00u) dm = max(dm, hi);
+            }
+#pragma unroll
+            for (int x = 1; x < 64; x *= 2) dm = max(dm, (uint32_t)__shfl_xor((int)dm, x, 64));
+            // 2^en ≥ every scale: one above the exponent, or of a subnormal its bit length − 24
+            const int en = dm >= 0x400u ? (int)(dm >> 10) - 14 : 8 - (dm ? __builtin_clz(dm) : 32);
+            const int ed_n = max(ed, __builtin_amdgcn_readfirstlane(en));
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                // the reference is the largest score + ed − 7
+                const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (float)(ed - 7);
+                const float top = fmaxf(best, max_over_keys(mx[n]));
+                const float ref_n = top <= KV_NONE ? KV_NONE : top + (float)(ed_n - 7);
+                const float alpha = ref_n == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - ref_n);
+                ref[n] = ref_n;
+                sum[n] *= alpha;
+#pragma unroll
+                for (int w = 0; w < W; w++) acc[n][w] *= alpha;
+            }
+            ed = ed_n;
+        }
+
+        // ---- probabilities, in units of the reference
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                t[n][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(t[n][j], c1[n], -ref[n]));
+                sum[n] += t[n][j];
+            }
+
+        // ---- Oᵀ += Vᵀ·(P·d)ᵀ, block by block of V's channels
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const kv_h8 vw[2] = {vword(2 * b), vword(2 * b + 1)};
+            kv_u4 p[NT][PARTS];
+            kv_u4 d = vscale(b);
+            if (special) {
+                uint32_t h = all;
+                __asm__ volatile("" : "+v"(h));  // (nothing of this ahead of the branch)
+#pragma unroll
+                for (int j = 0; j < 4; j++) d[j] &= keep_pair(h, j);
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (!F32) {
+                        p[n][0][j] = scaled_pair(t[n][2 * j], t[n][2 * j + 1], d[j]);
+                    } else {
+                        const kv_h2 dd = as_h2(d[j]);
+                        float x = t[n][2 * j] * (float)dd[0], y = t[n][2 * j + 1] * (float)dd[1];
+                        // one value for hi and for lo: folded into a mixed fma, hi alone would be rounded from the exact product
+                        __asm__("" : "+v"(x), "+v"(y));
+                        const kv_h2 hi = {(_Float16)x, (_Float16)y};
+                        p[n][0][j] = __builtin_bit_cast(uint32_t, hi);
+                        p[n][PARTS - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
+                    }
+                }
+            if (NT > 1 && partly) {
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t h = hidden[n];
+                    __asm__ volatile("" : "+v"(h));  // (nothing of this ahead of the branch)
+#pragma unroll
+                    for (int x = 0; x < PARTS; x++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) p[n][x][j] &= keep_pair(h, j);
+                }
+            }
+#pragma unroll
+            for (int w = 2 * b; w < 2 * b + 2; w++)
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if constexpr (!F32) {
-                            p[n][0][j] = scaled_pair(t[n][2 * j], t[n][2 * j + 1], d[j]);
-                        } else {
-                            const kv_h2 dd = as_h2(d[j]);
-                            float x = t[n][2 * j] * (float)dd[0], y = t[n][2 * j + 1] * (float)dd[1];
-                            // one value for hi and for lo: folded into a mixed fma, hi alone would be rounded from the exact product
-                            __asm__("" : "+v"(x), "+v"(y));
-                            const kv_h2 hi = {(_Float16)x, (_Float16)y};
-                            p[n][0][j] = __builtin_bit_cast(uint32_t, hi);
-                            p[n][PARTS - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
-                        }
-                    }
-                if (NT > 1 && partly) {
-                    __asm__ volatile("");  // (a branch, not selects)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int x = 0; x < PARTS; x++)
-#pragma unroll
-                            for (int j = 0; j < 4; j++) p[n][x][j] &= keep_pair(hidden[n], j);
-                }
-#pragma unroll
-                for (int w = 2 * b; w < 2 * b + 2; w++) {
-                    const kv_h8 vw = V.word(w, M);
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int x = 0; x < PARTS; x++)
-                            acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw, __builtin_bit_cast(kv_h8, p[n][x]), acc[n][w], 0, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (!more) break;
-            V.load(pn + C::HALF, lane);
-#pragma unroll
-            for (int i = 0; i < VD; i++)
-                vds[i] = *(const uint32_t *)(pn + C::HALF + C::CODES + ((lane + 64 * i) % (NB * 16)) * 4);
-            g = gn;
-            have = have_n;
+                    for (int x = 0; x < PARTS; x++)
+                        acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw[w & 1], __builtin_bit_cast(kv_h8, p[n][x]), acc[n][w], 0, 0, 0);
+            if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
     }
 
-    // ---- the four waves joined: 2 and 3 into 0 and 1, then 1 into 0
+    __device__ __forceinline__ void join_lanes() {
 #pragma unroll
-    for (int n = 0; n < NT; n++) sum[n] = sum_over_keys(sum[n]);
-    auto give = [&](int slot) {
+        for (int n = 0; n < NT; n++) sum[n] = sum_over_keys(sum[n]);
+    }
+
+    // Accumulators and sums through LDS (`at` by lane, NT · (W · 1024 + 512) bytes
+    // of a wave) into another wave's of the same columns.
+    __device__ __forceinline__ void give(uint8_t *at, int lane) const {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            lds_ml[slot][n][0][lane] = ref[n];
-            lds_ml[slot][n][1][lane] = sum[n];
 #pragma unroll
-            for (int w = 0; w < W; w++) lds[slot][n * W + w][lane] = acc[n][w];
+            for (int w = 0; w < W; w++) *(kv_f4 *)(at + (n * W + w) * 1024) = acc[n][w];
+            *(float2 *)(at - lane * 8 + NT * W * 1024 + n * 512) = make_float2(ref[n], sum[n]);
         }
-    };
-    auto take = [&](int slot) {
+    }
+    __device__ __forceinline__ void take(const uint8_t *at, int lane) {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            const float r = lds_ml[slot][n][0][lane], l = lds_ml[slot][n][1][lane];
-            const float top = fmaxf(ref[n], r);
+            const float2 o = *(const float2 *)(at - lane * 8 + NT * W * 1024 + n * 512);
+            const float top = fmaxf(ref[n], o.x);
             const float wa = ref[n] == top ? 1.f : __builtin_amdgcn_exp2f(ref[n] - top);
-            const float wb = r == top ? 1.f : __builtin_amdgcn_exp2f(r - top);
+            const float wb = o.x == top ? 1.f : __builtin_amdgcn_exp2f(o.x - top);
             ref[n] = top;
-            sum[n] = sum[n] * wa + l * wb;
+            sum[n] = sum[n] * wa + o.y * wb;
 #pragma unroll
-            for (int w = 0; w < W; w++) acc[n][w] = acc[n][w] * wa + lds[slot][n * W + w][lane] * wb;
+            for (int w = 0; w < W; w++) acc[n][w] = acc[n][w] * wa + *(const kv_f4 *)(at + (n * W + w) * 1024) * wb;
         }
+    }
+
+    // The columns' rows of o, or their part of a key range.
+    __device__ __forceinline__ void store(const KvAttnArgs &a, const KvTask &k, int lane) const {
+        const int col = lane & 15, ka = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            if (c0 + 16 * n + col >= k.ncols) continue;
+            const int64_t row = (int64_t)tok[n] * a.nh + head[n];
+            if (a.nsplit > 1) {
+                const int64_t at = (int64_t)k.split * a.n_tokens * a.nh + row;
+                float *o = a.part_o + at * D + 4 * ka;
+#pragma unroll
+                for (int w = 0; w < W; w++) *(kv_f4 *)(o + 16 * w) = acc[n][w];
+                if (ka == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(ref[n], sum[n]);
+                continue;
+            }
+            const float inv = sum[n] == 0.f ? 0.f : 1.0f / sum[n];  // no key at all: zeros
+            if constexpr (F32) {
+                float *o = (float *)a.o + row * D + 4 * ka;
+#pragma unroll
+                for (int w = 0; w < W; w++) *(kv_f4 *)(o + 16 * w) = acc[n][w] * inv;
+            } else {
+                _Float16 *o = (_Float16 *)a.o + row * D + 4 * ka;
+#pragma unroll
+                for (int w = 0; w < W; w++) {
+                    const kv_f4 x = acc[n][w] * inv;
+                    *(kv_h4 *)(o + 16 * w) = kv_h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+                }
+            }
+        }
+    }
+};
+
+// ---- few columns: bound by the cache's bytes ---------------------------------
+// A work-group takes NT · 16 columns against one range of keys; its four waves
+// take chunks in turn and are joined in LDS.  Each wave keeps a ring of two
+// chunks in LDS, loaded straight into it: while one is worked on the next is
+// under way without holding registers, so that four work-groups share a CU.
+constexpr int KV_STAGES = 2, KV_WAVES = 4;
+// Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
+// through an accumulation register; more where the registers suffice.
+constexpr int kv_waves(int NB, int NT) { return NT > 1 || NB == 8 ? 2 : (NB <= 2 ? 4 : 3); }
+
+template <int Q, int NB, bool F32, int NT>
+__global__ __launch_bounds__(64 * KV_WAVES, kv_waves(NB, NT)) void k_kv_attn(KvAttnArgs a) {
+    using C = KvChunk<Q, NB>;
+    using Cols = KvColumns<NB, F32, NT, true>;
+    constexpr int W = Cols::W, WAVES = KV_WAVES;
+    constexpr int LD = (C::BYTES + 1023) / 1024;  // 1 KB loads of a chunk
+    // at the end the accumulators of two waves
+    constexpr int RING = WAVES * KV_STAGES * C::BYTES, JOIN = 2 * NT * (W * 1024 + 512);
+    __shared__ __attribute__((aligned(16))) uint8_t smem[RING > JOIN ? RING : JOIN];
+
+    const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int s;
+    const KvTask k = kv_task<16 * NT>(a, s);
+    if (!k.some) return;
+    const KvPlaces places(a, s, k.kvh, C::BYTES);
+
+    const int g_end = (k.k_end + 31) >> 5;
+    int g = (k.k_begin >> 5) + wave;
+    uint8_t *const ring = smem + wave * (KV_STAGES * C::BYTES);
+    // a chunk into a slot of the ring: LD loads, the last of fewer lanes
+    auto fetch = [&](const uint8_t *p, int slot) {
+#pragma unroll
+        for (int i = 0; i < LD; i++)
+            if (C::BYTES - i * 1024 >= 1024 || lane * 16 < C::BYTES - i * 1024)
+                __builtin_amdgcn_global_load_lds((const void *)(p + i * 1024 + lane * 16),
+                                                 (__attribute__((address_space(3))) void *)(ring + slot * C::BYTES + i * 1024), 16, 0, 0);
     };
-    if (wave >= 2) give(wave - 2);
+    bool has[KV_STAGES];  // whether the cache has the page of the chunk in a slot
+    const bool any = k.k_begin < k.k_end && g < g_end;
+    if (any) {
+#pragma unroll
+        for (int i = 0; i < KV_STAGES; i++) {
+            has[i] = true;
+            if (g + WAVES * i < g_end) fetch(places.at(g + WAVES * i, has[i]), i);
+        }
+    }
+    Cols cols;
+    cols.start(a, k, k.c0, lane);
+    if (any) {
+        int slot = 0;
+        while (true) {
+            // this chunk has arrived when no more loads are under way than the next one's
+            if (g + WAVES < g_end) __builtin_amdgcn_s_waitcnt(vm_wait(LD));
+            else __builtin_amdgcn_s_waitcnt(vm_wait(0));
+            __asm__ volatile("" ::: "memory");
+            const kv_lds kh = (kv_lds)(ring + slot * C::BYTES), vh = kh + C::HALF;
+            const bool have = has[0];
+            const bool more = g + WAVES * KV_STAGES < g_end;
+            bool have_n = true;
+            const uint8_t *pn = places.at(more ? g + WAVES * KV_STAGES : g, have_n);
+            KvHalf<Q, NB> K, V;
+            K.load(kh, lane);
+            cols.chunk(
+                a, k.len, g, have, lane, [&](int i) { return K.word(i, cols.M); },
+                [&](int b) { return scales_of<Q, NB>(kh, b, ka); },
+                [&](int i) {
+                    if (i == 0) V.load(vh, lane);
+                    return V.word(i, cols.M);
+                },
+                [&](int b) { return scales_of<Q, NB>(vh, b, ka); },
+                [&](int i) {
+                    return *(__attribute__((address_space(3))) const uint32_t *)(vh + C::CODES + ((lane + 64 * i) % (NB * 16)) * 4);
+                });
+            if (g + WAVES >= g_end) break;
+            // the slot's words are all in registers: the next chunk may come
+            if (more) fetch(pn, slot);
+#pragma unroll
+            for (int i = 0; i + 1 < KV_STAGES; i++) has[i] = has[i + 1];
+            has[KV_STAGES - 1] = have_n;
+            g += WAVES;
+            slot = slot + 1 < KV_STAGES ? slot + 1 : 0;
+        }
+    }
+    cols.join_lanes();
+
+    // the rings are done with: the memory joins the waves, 2 and 3 into 0 and 1, then 1 into 0
+    constexpr int ONE = NT * (W * 1024 + 512);
+    uint8_t *const at = smem + lane * 16;
     __syncthreads();
-    if (wave < 2) take(wave);
+    if (wave >= 2) cols.give(at + (wave - 2) * ONE, lane);
     __syncthreads();
-    if (wave == 1) give(0);
+    if (wave < 2) cols.take(at + wave * ONE, lane);
+    __syncthreads();
+    if (wave == 1) cols.give(at, lane);
     __syncthreads();
     if (wave != 0) return;
-    take(0);
-
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        if (c0 + 16 * n + col >= ncols) continue;
-        const int64_t row = (int64_t)tok[n] * a.nh + head[n];
-        if (a.nsplit > 1) {
-            const int64_t at = (int64_t)split * a.n_tokens * a.nh + row;
-            float *o = a.part_o + at * D + 4 * ka;
-#pragma unroll
-            for (int w = 0; w < W; w++) *(kv_f4 *)(o + 16 * w) = acc[n][w];
-            if (ka == 0) *(float2 *)(a.part_ml + at * 2) = make_float2(ref[n], sum[n]);
-            continue;
-        }
-        const float inv = sum[n] == 0.f ? 0.f : 1.0f / sum[n];  // no key at all: zeros
-        if constexpr (F32) {
-            float *o = (float *)a.o + row * D + 4 * ka;
-#pragma unroll
-            for (int w = 0; w < W; w++) *(kv_f4 *)(o + 16 * w) = acc[n][w] * inv;
-        } else {
-            _Float16 *o = (_Float16 *)a.o + row * D + 4 * ka;
-#pragma unroll
-            for (int w = 0; w < W; w++) {
-                const kv_f4 x = acc[n][w] * inv;
-                *(kv_h4 *)(o + 16 * w) = kv_h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
-            }
-        }
-    }
+    cols.take(at, lane);
+    cols.store(a, k, lane);
 }
 
-// Columns tiles a wave holds: as many as its registers leave room for (the
-// accumulators are 8·NB of them a tile), one where there are no more columns.
+// ---- many columns: bound by vector instructions ------------------------------
+// Eight waves: KS streams of them take every KS-th chunk, and the waves of a
+// stream hold columns of their own against the same chunks, whose words are
+// converted to fp16 once for all of them: each converts some while the chunk
+// before is worked on, into one of two buffers of whole MFMA operands (16 bytes
+// a lane and word, in the order of lanes, so neither side has bank conflicts).
+// One barrier a chunk.  Two streams halve the longest work-group (a causal
+// prompt's last columns see every key) and are joined in LDS; at head dim 256,
+// where that memory holds one stream's buffers, all eight share one.
+constexpr int kv_tile_waves(int NB, bool F32) { return NB == 8 && !F32 ? 12 : 8; }
+constexpr int kv_tile_nt(int NB, bool F32) { return F32 ? (NB <= 2 ? 2 : 1) : (NB == 8 ? 1 : 2); }
+constexpr int kv_tile_fill(int NB, bool F32) { return F32 ? 2 : (NB <= 2 ? 4 : (NB == 8 ? 3 : 2)); }
+constexpr int kv_tile_streams(int NB) { return NB == 8 ? 1 : 2; }
+constexpr int kv_tile_cols(int NB, bool F32) { return 16 * kv_tile_nt(NB, F32) * kv_tile_waves(NB, F32) / kv_tile_streams(NB); }
+
+template <int Q, int NB, bool F32>
+__global__ __launch_bounds__(64 * kv_tile_waves(NB, F32), kv_tile_fill(NB, F32)) void k_kv_attn_tile(KvAttnArgs a) {
+    using C = KvChunk<Q, NB>;
+    constexpr int NT = kv_tile_nt(NB, F32), KS = kv_tile_streams(NB), CG = kv_tile_waves(NB, F32) / KS;
+    using Cols = KvColumns<NB, F32, NT, (NB > 4 || (!F32 && NB <= 2))>;
+    constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
+    constexpr int W = Cols::W, BUFS = 2 * KS * BUF, JOIN = KS > 1 ? CG * NT * (W * 1024 + 512) : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[BUFS > JOIN ? BUFS : JOIN];
+
+    const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ks = wave / CG, cg = wave % CG, st = tid % (64 * CG);  // stream, column group, thread of the stream
+    int s;
+    const KvTask k = kv_task<kv_tile_cols(NB, F32)>(a, s);
+    if (!k.some) return;
+    const KvPlaces places(a, s, k.kvh, C::BYTES);
+
+    // pieces of K and V this wave converts, and the scales (16 bytes a thread)
+    constexpr int PW = (2 * C::PIECES + CG - 1) / CG;
+    static_assert(8 * NB <= 64 * CG, "a thread for every 16 bytes of scales");
+    uint4 raw[PW], rawd;
+    auto fetch = [&](const uint8_t *p) {
+#pragma unroll
+        for (int i = 0; i < PW; i++) {
+            const int u = cg + i * CG, pi = u % C::PIECES;
+            if (u >= 2 * C::PIECES) continue;
+            const uint8_t *q = p + (u / C::PIECES) * C::HALF + pi * 1024 + lane * (C::width(pi) * Q);
+            if (C::width(pi) == C::PER) {
+                raw[i] = gload16(q);
+            } else {
+                const uint2 x = gload8(q);
+                raw[i] = make_uint4(x.x, x.y, 0, 0);
+            }
+        }
+        if (st < 8 * NB) rawd = gload16(p + C::CODES + (st < 4 * NB ? st * 16 : C::HALF + (st - 4 * NB) * 16));
+    };
+    const KvMagic M;
+    auto convert = [&](uint8_t *buf) {
+#pragma unroll
+        for (int i = 0; i < PW; i++) {
+            const int u = cg + i * CG, pi = u % C::PIECES;
+            if (u >= 2 * C::PIECES) continue;
+            uint8_t *o = buf + (u / C::PIECES) * HALF + pi * (C::PER * 1024) + lane * 16;
+            const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int w = 0; w < C::PER; w++) {
+                if (w >= C::width(pi)) continue;
+                kv_h8 h;
+                if constexpr (Q == 4) h = word_h8_q4(x[w], M);
+                else h = word_h8_q8(x[2 * w], x[2 * w + 1]);
+                *(kv_h8 *)(o + w * 1024) = h;
+            }
+        }
+        if (st < 8 * NB) *(uint4 *)(buf + 2 * HALF + st * 16) = rawd;
+    };
+
+    // every stream makes `turns` turns, the last maybe without a chunk
+    const int g0 = k.k_begin >> 5, g_end = (k.k_end + 31) >> 5;
+    const int turns = k.k_begin < k.k_end ? (g_end - g0 + KS - 1) / KS : 0;
+    int g = g0 + ks;
+    bool have = true, have_n = true;
+    if (turns > 0 && g < g_end) fetch(places.at(g, have));
+    Cols cols;
+    cols.start(a, k, k.c0 + cg * (16 * NT), lane);
+    // this wave's own columns see no key from here on
+    const int i_last = (min(cols.c0 + 16 * NT, k.ncols) - 1) / k.G;
+    const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.len - k.nq + i_last + 1 : k.len);
+    uint8_t *const mine = smem + ks * BUF;  // buffer t of the stream at t · KS · BUF
+    if (turns > 0) {
+        if (g < g_end) convert(mine);
+        if (g + KS < g_end) fetch(places.at(g + KS, have_n));
+        __syncthreads();
+        for (int t = 0; t < turns; t++, g += KS) {
+            const kv_lds kb = (kv_lds)(mine + (t & 1) * (KS * BUF)), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
+            bool have_2 = have_n;
+            if (g + KS < g_end) {
+                convert(mine + (~t & 1) * (KS * BUF));
+                if (g + 2 * KS < g_end) fetch(places.at(g + 2 * KS, have_2));
+            }
+            if (32 * g < see_any)
+                cols.chunk(
+                    a, k.len, g, have, lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
+                    [&](int b) { return lds16(kd + b * 64 + ka * 16); },
+                    [&](int i) { return __builtin_bit_cast(kv_h8, lds16(vb + i * 1024 + lane * 16)); },
+                    [&](int b) { return lds16(vd + b * 64 + ka * 16); },
+                    [&](int i) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + ((lane + 64 * i) % (NB * 16)) * 4); });
+            __syncthreads();
+            have = have_n;
+            have_n = have_2;
+        }
+    }
+    cols.join_lanes();
+    if constexpr (KS > 1) {
+        // the second stream's sums into the first's (the last barrier left the buffers free)
+        uint8_t *const at = smem + cg * (NT * (W * 1024 + 512)) + lane * 16;
+        if (ks == 1) cols.give(at, lane);
+        __syncthreads();
+        if (ks == 1) return;
+        cols.take(at, lane);
+    }
+    if (cols.c0 < k.ncols) cols.store(a, k, lane);
+}
+
+// Column tiles a wave of the first kernel holds where there are more than 16 columns.
 template <int NB, bool F32>
-constexpr int kv_most_tiles() { return NB <= 2 ? (F32 ? 2 : 4) : (NB == 8 ? 1 : 2); }
+constexpr int kv_most_tiles() { return NB == 8 ? 1 : 2; }
 
 template <int Q>
 hipError_t launch_kv_attn(const KvAttnArgs &a, bool f32, hipStream_t st) {
-    const int64_t units = (int64_t)a.n_seq * a.c.heads * a.nsplit;
-    const int64_t grid = (units >= 8 ? (units + 7) / 8 * 8 : units) * a.ctiles;
+    const int64_t grid = ((int64_t)a.n_seq * a.c.heads * a.nsplit * a.ctiles + 7) / 8 * 8;
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     auto go = [&](auto nb, auto f) {
         constexpr int NB = nb(), MOST = kv_most_tiles<NB, f()>();
-        if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), dim3((unsigned)grid), dim3(256), 0, st, a);
-        else if (a.nt == MOST) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), MOST>), dim3((unsigned)grid), dim3(256), 0, st, a);
+        const dim3 g((unsigned)grid);
+        if (a.tile) hipLaunchKernelGGL((k_kv_attn_tile<Q, NB, f()>), g, dim3(64 * kv_tile_waves(NB, f())), 0, st, a);
+        else if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), g, dim3(64 * KV_WAVES), 0, st, a);
+        else if (a.nt == MOST) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), MOST>), g, dim3(64 * KV_WAVES), 0, st, a);
         else return hipErrorInvalidValue;
         return hipGetLastError();
     };

@@ -91,20 +91,17 @@ int check_batch(const char *fn, const s3e_kv_cache *c, const s3e_kv_batch *b, in
     return S3E_OK;
 }
 
-// Work-groups a call aims at: enough waves on every CU to keep HBM busy.
-constexpr int64_t KV_WGS = 768;
 // Fewest keys a work-group is worth starting for.
 constexpr int64_t KV_MIN_KEYS = 256;
 
-// The column tiles and the split over keys: by the host's bounds alone, so that
-// a captured call is the same for any lengths.
+// The kernel, its column tiles and the split over keys: by the host's bounds
+// alone, so that a captured call is the same for any lengths.
 void plan(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, bool f32, KvAttnArgs &a) {
-    const int64_t cols = b->max_q * (nh / c->n_heads);
-    a.nt = kv_attn_nt(c->type, c->head_dim, f32, cols);
-    a.ctiles = (int)((cols + 16 * a.nt - 1) / (16 * a.nt));
+    a.n_seq = (int)b->n_seq;
+    kv_attn_columns(a, c->head_dim, f32, b->max_q * (nh / c->n_heads));
     const int64_t wgs = b->n_seq * c->n_heads * a.ctiles;
-    int64_t ns = std::min((KV_WGS + wgs - 1) / wgs, (b->max_kv + KV_MIN_KEYS - 1) / KV_MIN_KEYS);
-    ns = std::max<int64_t>(ns, 1);
+    int64_t ns = a.tile ? a.goal / wgs : (a.goal + wgs - 1) / wgs;
+    ns = std::max<int64_t>(1, std::min(ns, (b->max_kv + KV_MIN_KEYS - 1) / KV_MIN_KEYS));
     a.chunk = std::max<int64_t>(128, round_up((b->max_kv + ns - 1) / ns, 128));
     a.nsplit = (int)std::max<int64_t>(1, (b->max_kv + a.chunk - 1) / a.chunk);
 }
@@ -230,10 +227,9 @@ extern "C" int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_bat
     a.mask_ld = mask_ld;
     a.mask_vec = (uintptr_t)mask % 16 == 0 && mask_ld % 8 == 0;
     a.o = o;
-    a.scale = (float)(std::fabs((double)scale) * 1.4426950408889634);
-    a.neg = scale < 0;
+    a.sign = scale < 0 ? -1 : (scale > 0 ? 1 : 0);
+    a.scale = a.sign ? std::max((float)(std::fabs((double)scale) * 1.4426950408889634), 1.17549435e-38f) : 1.0f;
     a.causal = causal != 0;
-    a.n_seq = (int)b->n_seq;
     a.n_tokens = (int)b->n_tokens;
     a.max_q = (int)std::min(b->max_q, b->n_tokens);
     a.nh = (int)nh;

@@ -316,6 +316,43 @@ def test_attention(ctx, t, io, heads, nh, D, page, lens, more):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("form", ["few", "more", "many", "split"])
+def test_every_kernel(ctx, t, io, D, form):
+    # up to 16, up to 32 and more columns a key/value head; many columns against several key ranges
+    heads, nh, lens, more = {"few": (2, 6, [(3, 300), (2, 33)], {}), "more": (1, 3, [(9, 290), (7, 7)], {"mask": True}),
+                             "many": (1, 3, [(90, 300), (37, 37), (50, 12)], {}),
+                             "split": (1, 1, [(140, 900)], {"mask": True, "causal": False})}[form]
+    print(t, io, D, form, flush=True)
+    x = Batch(ctx, t, io, heads, nh, D, 64, lens, seed=D + len(form), **more)
+    assert form != "split" or s3e.kv_attn_workspace(x.c, x.b, nh, io) > 0
+    x.check()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D,nq", [(64, 2), (64, 20), (64, 70), (128, 70), (256, 40)])
+def test_a_key_hidden_from_some_queries(ctx, t, io, D, nq):
+    # its NaN reaches the queries that see it and no others, though lanes hold columns of both kinds
+    kv = 100
+    x = Batch(ctx, t, io, 1, 1, D, 64, [(nq, kv)], seed=nq, mask=True, causal=False)
+    x.mask[:] = 0
+    x.mask[::2, 33] = -np.inf
+    x.mask[1::3, 70:80] = -np.inf
+    x.md.upload(x.mask)
+    table = x.arrays[2].download(np.int32, (1, 2))
+    slots = np.array([table[0, j // 64] * 64 + j % 64 for j in range(kv)], np.int32)
+    k, v = x.k.copy(), x.v.copy()
+    v[33] = np.nan
+    ctx.kv_write(x.c, s3e.TYPE_F32, ctx.to_device(k), (D, D), ctx.to_device(v), (D, D), ctx.to_device(slots), kv)
+    got = x.run()
+    want, bound = x.want()  # (of the rows that do not see key 33: its value has no part in them)
+    assert np.isnan(got[1::2]).all()
+    assert (np.abs(got[::2].astype(np.float64) - want[::2]) <= bound[::2]).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_pairs_are_whole(ctx, t):
     # the high half of every fp32 pair is the one its low half completes: 40 x 10^4 products a call, ties among them
     for seed in range(6):

@@ -7,83 +7,146 @@ namespace {
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
-// Eight consecutive values of a row.
+// Maximum and minimum as the one instruction they are (the builtins put another
+// before it that quiets a signalling NaN; whether there is a NaN is seen apart).
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ float max_of(float a, float b) { float r; __asm__("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ float min_of(float a, float b) { float r; __asm__("v_min_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ h2 max_of(h2 a, h2 b) { h2 r; __asm__("v_pk_max_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+__device__ __forceinline__ h2 min_of(h2 a, h2 b) { h2 r; __asm__("v_pk_min_f16 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b)); return r; }
+
+// Before lane exchanges (DPP) of what inline asm has written: two wait states,
+// which the compiler puts only behind instructions of its own.
+__device__ __forceinline__ void settle(float &a, float &b) { __asm__("s_nop 1" : "+v"(a), "+v"(b)); }
+
+// Eight consecutive values of a row, as they lie in memory until they are used.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, int vec, float *v) {
-    if constexpr (sizeof(T) == 2) {
+struct Raw8 {
+    T x[8];
+    __device__ __forceinline__ void load(const T *p, int vec) {
         if (vec) {
-            const h8 x = *(const h8 *)p;
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = (float)x[j];
-            return;
-        }
-    } else {
-        if (vec) {
-            const float4 x = *(const float4 *)p, y = *(const float4 *)(p + 4);
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-            v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-            return;
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) *(uint4 *)(x + i * (16 / sizeof(T))) = ((const uint4 *)p)[i];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] = p[j];
         }
     }
+    // largest and smallest value, and a number only if all of them are
+    __device__ __forceinline__ void range(float &hi, float &lo, float &odd) const {
+        if constexpr (sizeof(T) == 2) {
+            h2 v[4], z = {(_Float16)0.f, (_Float16)0.f};
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = (float)p[j];
-}
+            for (int j = 0; j < 4; j++) {
+                v[j] = h2{x[2 * j], x[2 * j + 1]};
+                z = __builtin_elementwise_fma(v[j], h2{(_Float16)0.f, (_Float16)0.f}, z);
+            }
+            const h2 a = max_of(max_of(v[0], v[1]), max_of(v[2], v[3])), b = min_of(min_of(v[0], v[1]), min_of(v[2], v[3]));
+            hi = max_of((float)a[0], (float)a[1]);
+            lo = min_of((float)b[0], (float)b[1]);
+            odd = (float)z[0] + (float)z[1];
+        } else {
+            hi = lo = x[0];
+            odd = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                hi = max_of(hi, x[j]);
+                lo = min_of(lo, x[j]);
+                odd = __builtin_fmaf(x[j], 0.f, odd);
+            }
+        }
+    }
+    // the first value of magnitude top: its place, or 8
+    __device__ __forceinline__ int place(float top) const {
+        int at = 8;
+#pragma unroll
+        for (int j = 7; j >= 0; j--) at = fabsf((float)x[j]) == top ? j : at;
+        return at;
+    }
+};
 
 // The codes of one 32-channel block held as 8 values by each of 4 neighbouring
 // lanes (in channel order), as ggml's quantize_row_q4_0 (d = max / −8, max the
 // first value of largest magnitude; q = min(15, ⌊x/d + 8.5⌋)) and the engine's
 // Q8_0 conversion (d = amax / 127, q = round-half-even(x·(127/amax))) choose
 // them in fp32.  A block with an infinity or a NaN gets a NaN scale, so that
-// all of it reads back as NaN.  codes: bytes 0..15, or int8 bits.
-template <int Q>
-__device__ __forceinline__ void quant_block(const float *v, int lane, uint32_t *codes, uint16_t &scale) {
-    uint32_t top = 0;
-    float lead = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const uint32_t a = __float_as_uint(v[j]) & 0x7fffffffu;
-        if (a > top) {
-            top = a;
-            lead = v[j];
-        }
-    }
-#pragma unroll
-    for (int x = 1; x <= 2; x *= 2) {
-        const uint32_t ot = __shfl_xor(top, x, 64);
-        const float ol = __shfl_xor(lead, x, 64);
-        if (ot > top || (ot == top && (lane & x))) {
-            top = ot;
-            lead = ol;
-        }
-    }
-    const bool finite = top < 0x7f800000u;
+// all of it reads back as NaN, and the codes of zeros.  codes: 0..15, or int8
+// in the low byte.
+// (Lane exchanges within four lanes are DPP moves, folded into the instruction
+// that uses them.)
+template <int X>
+__device__ __forceinline__ int quad_xor(int v) {
+    static_assert(X == 1 || X == 2, "of four lanes");
+    return __builtin_amdgcn_update_dpp(v, v, X == 1 ? 0xb1 : 0x4e, 0xf, 0xf, true);
+}
+template <int X>
+__device__ __forceinline__ float quad_xor(float v) { return __int_as_float(quad_xor<X>(__float_as_int(v))); }
+
+template <int Q, typename T>
+__device__ __forceinline__ void quant_block(const Raw8<T> &raw, int lane, uint32_t *codes, uint16_t &scale) {
+    float hi, lo, odd;
+    raw.range(hi, lo, odd);
+    settle(hi, lo);
+    hi = max_of(hi, quad_xor<1>(hi)), lo = min_of(lo, quad_xor<1>(lo)), odd += quad_xor<1>(odd);
+    settle(hi, lo);
+    hi = max_of(hi, quad_xor<2>(hi)), lo = min_of(lo, quad_xor<2>(lo)), odd += quad_xor<2>(odd);
+    const float top = max_of(hi, -lo);
     float d, id;
     if constexpr (Q == 4) {
-        d = lead / -8.0f;
+        float lead = hi > -lo ? hi : lo;
+        if (hi == -lo && top != 0.f) {
+            // both signs reach it: the first in the block decides
+            const int mine = raw.place(top), at = mine == 8 ? 32 : (lane & 3) * 8 + mine;
+            int first = min(at, quad_xor<1>(at));
+            first = min(first, quad_xor<2>(first));
+            int sign = 0;  // of the lane that holds it: 1 where it is negative
+#pragma unroll
+            for (int j = 0; j < 8; j++) sign = first == (lane & 3) * 8 + j && raw.x[j] < (T)0.f ? 1 : sign;
+            sign |= quad_xor<1>(sign);
+            sign |= quad_xor<2>(sign);
+            lead = sign ? -top : top;
+        }
+        d = (top == 0.f ? 0.f : lead) * -0.125f;
         id = d != 0.f ? 1.0f / d : 0.f;
     } else {
-        const float amax = __uint_as_float(top);
-        d = amax / 127.0f;
-        id = top ? 127.0f / amax : 0.f;
+        d = top / 127.0f;
+        id = top != 0.f ? 127.0f / top : 0.f;
     }
     // (a scale whose reciprocal overflows is far below fp16's smallest: zero)
-    if (!finite || __builtin_isinf(id)) id = 0.f;
-    scale = finite ? half_bits(d) : (uint16_t)0x7e00;
+    if (__builtin_isinf(id)) id = 0.f;
+    scale = half_bits(d);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-        const float x = finite ? v[j] * id : 0.f;
-        if constexpr (Q == 4) codes[j] = (uint32_t)min(15, (int)(x + 8.5f));
-        else codes[j] = (uint32_t)(int)__builtin_rintf(x) & 0xffu;
+        float x = __builtin_fmaf((float)raw.x[j], id, 0.f);  // the rounded product (of fp16 as it is)
+        __asm__("" : "+v"(x));
+        if constexpr (Q == 4) codes[j] = min(15u, (uint32_t)(x + 8.5f));
+        else codes[j] = __float_as_uint(x + 12582912.0f);  // 1.5 · 2^23: rounded half to even into the low bits
     }
+    if (!(odd == 0.f)) {
+        scale = 0x7e00;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            codes[j] = Q == 4 ? 8 : 0;
+            __asm__ volatile("" : "+v"(codes[j]));  // (a branch, not selects)
+        }
+    }
+}
+
+// Bytes 0 of four words as one.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
 }
 
 template <int Q>
 __device__ __forceinline__ uint64_t pack_word(const uint32_t *c) {
-    uint64_t x = 0;
+    if constexpr (Q == 4) {
+        uint32_t x = c[0];
 #pragma unroll
-    for (int j = 0; j < 8; j++)
-        x |= (uint64_t)c[j] << (Q == 4 ? 4 * ((j >> 1) + 4 * (j & 1)) : 8 * j);
-    return x;
+        for (int j = 1; j < 8; j++) x |= c[j] << (4 * ((j >> 1) + 4 * (j & 1)));
+        return x;
+    } else {
+        return pack4(c[0], c[1], c[2], c[3]) | (uint64_t)pack4(c[4], c[5], c[6], c[7]) << 32;
+    }
 }
 
 template <int Q>
@@ -121,6 +184,17 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
     const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
     const int64_t r0 = (int64_t)blockIdx.x * KV_ROWS;
+    const T *x = (const T *)(is_v ? a.x[1] : a.x[0]);
+    const int64_t st = is_v ? a.st[1] : a.st[0], sh = is_v ? a.sh[1] : a.sh[0];
+    const int vec = is_v ? a.vec[1] : a.vec[0];
+    const int g = tid & 3;
+    // own rows, on their way while the slots are looked at
+    Raw8<T> own_row[NB];
+    {
+        const int64_t r = min(r0 + (tid >> 2), (int64_t)a.n - 1);
+#pragma unroll
+        for (int b = 0; b < NB; b++) own_row[b].load(x + r * st + head * sh + 32 * b + 8 * g, vec);
+    }
     if (tid < KV_ROWS + 21) {
         const int64_t r = r0 + tid - 7;
         int32_t s = -1;
@@ -144,17 +218,9 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
         }
         return ok;
     };
-    const T *x = (const T *)(is_v ? a.x[1] : a.x[0]);
-    const int64_t st = is_v ? a.st[1] : a.st[0], sh = is_v ? a.sh[1] : a.sh[0];
-    const int vec = is_v ? a.vec[1] : a.vec[0];
-    const int g = tid & 3;
-
     if (!is_v) {
         const int r = tid >> 2, s = sl[r + 7];
         if (s < 0) return;  // (the four lanes of a row together)
-        float v[NB][8];
-#pragma unroll
-        for (int b = 0; b < NB; b++) load8<T>(x + (r0 + r) * st + head * sh + 32 * b + 8 * g, vec, v[b]);
         uint8_t *ck = chunk_of(a.c, s, head, C::BYTES);
         const int key = s & 31, t = (key >> 2) & 1, row = 4 * (key >> 3) + (key & 3);
         uint64_t w[NB];
@@ -162,7 +228,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
         for (int b = 0; b < NB; b++) {
             uint32_t c[8];
             uint16_t d;
-            quant_block<Q>(v[b], lane, c, d);
+            quant_block<Q>(own_row[b], lane, c, d);
             w[b] = pack_word<Q>(c);
             if (g == (b & 3)) *(uint16_t *)(ck + C::CODES + (b * 32 + key) * 2) = d;
         }
@@ -183,30 +249,19 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
     }
 
     // V: own rows, then those of the next work-group that a run from here ends in
-    auto convert = [&](int r, bool own) {
+    auto convert = [&](int r, bool own, const Raw8<T> *raw) {
         const int s = sl[r + 7];
-        if (s < 0) return;
         const bool run = in_run(r);
-        if (!own && !(run && r - (s & 7) < KV_ROWS)) return;
-        float v[NB][8];
-#pragma unroll
-        for (int b = 0; b < NB; b++) load8<T>(x + (r0 + r) * st + head * sh + 32 * b + 8 * g, vec, v[b]);
         uint8_t *cv = chunk_of(a.c, s, head, C::BYTES) + C::HALF;
         const int key = s & 31;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             uint32_t c[8];
             uint16_t d;
-            quant_block<Q>(v[b], lane, c, d);
+            quant_block<Q>(raw[b], lane, c, d);
             if (own && g == (b & 3)) *(uint16_t *)(cv + C::CODES + (b * 32 + key) * 2) = d;
             if (run) {
-                uint2 y = make_uint2(0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    y.x |= c[j] << (8 * j);
-                    y.y |= c[4 + j] << (8 * j);
-                }
-                *(uint2 *)(codes_lds + r * D + 32 * b + 8 * g) = y;
+                *(uint2 *)(codes_lds + r * D + 32 * b + 8 * g) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -223,8 +278,16 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
             }
         }
     };
-    convert(tid >> 2, true);
-    if (tid < 28) convert(KV_ROWS + (tid >> 2), false);
+    if (sl[(tid >> 2) + 7] >= 0) convert(tid >> 2, true, own_row);
+    if (tid < 28) {
+        const int r = KV_ROWS + (tid >> 2), s = sl[r + 7];
+        if (s >= 0 && in_run(r) && r - (s & 7) < KV_ROWS) {
+            Raw8<T> next[NB];
+#pragma unroll
+            for (int b = 0; b < NB; b++) next[b].load(x + (r0 + r) * st + head * sh + 32 * b + 8 * g, vec);
+            convert(r, false, next);
+        }
+    }
     if (tid < 64) {
         const bool first = (sl[tid + 7] & 7) == 0 && in_run(tid);
         const uint64_t m = __ballot(first);
@@ -232,102 +295,197 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
         if (tid == 0) starts[0] = __popcll(m);
     }
     __syncthreads();
-    // whole words: unit (run, piece, channel m of 16)
-    const int units = starts[0] * C::PIECES * 16;
+    // whole words: unit (run, piece, four channels 4q .. 4q + 4 of 16).  The bytes
+    // of four channels come as one word a row; two rows' nibbles share its bytes,
+    // and a 4 × 4 transpose of bytes turns four such words into a channel's each
+    constexpr int ROWS = Q == 4 ? 2 : 1, WORDS4 = 8 / ROWS;  // rows in a byte, 4-byte words of eight rows
+    const int units = starts[0] * C::PIECES * 4;
     for (int u = tid; u < units; u += 256) {
-        const int m = u & 15, pi = (u >> 4) % C::PIECES, r = starts[1 + (u >> 4) / C::PIECES];
+        const int q = u & 3, pi = (u >> 2) % C::PIECES, r = starts[1 + (u >> 2) / C::PIECES];
         const int s = sl[r + 7];
         uint8_t *cv = chunk_of(a.c, s, head, C::BYTES) + C::HALF;
-        const int lane16 = 16 * ((s & 31) >> 3) + m;
-        uint64_t w[C::PER];
+        uint32_t out[4][4];  // channel, 4 bytes of its piece
 #pragma unroll
         for (int i = 0; i < C::PER; i++) {
-            const int ww = pi * C::PER + i;
-            uint32_t c[8];
+            const int w = min(pi * C::PER + i, C::WORDS - 1);  // (a short piece's missing words: any)
+            uint32_t in[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) c[j] = ww < C::WORDS ? codes_lds[(r + j) * D + 16 * ww + m] : 0;
-            w[i] = pack_word<Q>(c);
+            for (int j = 0; j < 8; j++) in[j] = *(const uint32_t *)(codes_lds + (r + j) * D + 16 * w + 4 * q);
+            uint32_t m[WORDS4];
+            if constexpr (Q == 4) m[0] = in[0] | in[2] << 4, m[1] = in[4] | in[6] << 4, m[2] = in[1] | in[3] << 4, m[3] = in[5] | in[7] << 4;
+            else
+#pragma unroll
+                for (int j = 0; j < 8; j++) m[j % WORDS4] = in[j];
+#pragma unroll
+            for (int h = 0; h < WORDS4 / 4; h++) {
+                const uint32_t a0 = __builtin_amdgcn_perm(m[4 * h + 1], m[4 * h], 0x05010400u), a1 = __builtin_amdgcn_perm(m[4 * h + 1], m[4 * h], 0x07030602u);
+                const uint32_t b0 = __builtin_amdgcn_perm(m[4 * h + 3], m[4 * h + 2], 0x05010400u), b1 = __builtin_amdgcn_perm(m[4 * h + 3], m[4 * h + 2], 0x07030602u);
+                const int at = i * (C::WB / 4) + h;
+                out[0][at] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+                out[1][at] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+                out[2][at] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+                out[3][at] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+            }
         }
-        if (C::width(pi) == C::PER) {
-            uint4 y;
-            if constexpr (Q == 4) y = make_uint4((uint32_t)w[0], (uint32_t)w[1], (uint32_t)w[2], (uint32_t)w[3]);
-            else y = make_uint4((uint32_t)w[0], (uint32_t)(w[0] >> 32), (uint32_t)w[1], (uint32_t)(w[1] >> 32));
-            *(uint4 *)(cv + C::word(pi * C::PER, lane16)) = y;
-        } else {
 #pragma unroll
-            for (int i = 0; i < C::PER; i++)
-                if (i < C::width(pi)) store_word<Q>(cv + C::word(pi * C::PER + i, lane16), w[i]);
+        for (int c = 0; c < 4; c++) {
+            uint8_t *o = cv + C::word(pi * C::PER, 16 * ((s & 31) >> 3) + 4 * q + c);
+            if (C::width(pi) == C::PER) *(uint4 *)o = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+            else *(uint2 *)o = make_uint2(out[c][0], out[c][1]);
         }
     }
 }
 
+// A code of a word as the byte of an int8.
 template <int Q>
-__device__ __forceinline__ int code_of(uint64_t w, int j) {
-    if constexpr (Q == 4) return (int)((w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15) - 8;
-    else return (int)(int8_t)(w >> (8 * j));
-}
-template <int Q>
-__device__ __forceinline__ uint64_t load_word(const uint8_t *p) {
-    if constexpr (Q == 4) return *(const uint32_t *)p;
-    else return *(const uint64_t *)p;
+__device__ __forceinline__ uint32_t code_of(uint64_t w, int j) {
+    if constexpr (Q == 4) return (((uint32_t)w >> (4 * ((j >> 1) + 4 * (j & 1)))) & 15u) - 8u;
+    else return (uint32_t)(w >> (8 * j));
 }
 
-// One tensor (blockIdx.z) of 64 rows and one head: thread 4r + g gives K's
-// channels 32b + 8g .. + 8 of row r (its words), or V's channels 16w + 4g .. + 4
-// (a code of each of their words; the eight rows of a run read the same words,
-// from L1).  A slot outside the cache reads as zeros.  Bound by HBM.
+// A lane's words of one piece (16 bytes of them, or the 8 of a last one).
+template <int Q, int NB>
+__device__ __forceinline__ void load_piece(const uint8_t *half, int p, int lane, uint64_t *w) {
+    using C = KvChunk<Q, NB>;
+    const uint8_t *at = half + C::word(p * C::PER, lane);
+    if (C::width(p) == C::PER) {
+        const uint4 x = gload16(at);
+        if constexpr (Q == 4) w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        else w[0] = x.x | (uint64_t)x.y << 32, w[1] = x.z | (uint64_t)x.w << 32;
+    } else {
+        const uint2 x = gload8(at);
+        w[0] = x.x, w[1] = x.y;
+    }
+}
+
+// Eight values of a row, each scale · code rounded once.
+template <typename T>
+__device__ __forceinline__ void store8(T *o, const float *v) {
+    if constexpr (sizeof(T) == 2) {
+        h8 z;
+#pragma unroll
+        for (int j = 0; j < 8; j++) z[j] = (_Float16)v[j];
+        *(h8 *)o = z;
+    } else {
+        *(float4 *)o = make_float4(v[0], v[1], v[2], v[3]);
+        *(float4 *)(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+
+// One tensor (blockIdx.z) of 64 rows and one head.  K: thread 4r + g gives
+// channels 32b + 8g .. + 8 of row r, its own words.  V's words hold eight keys
+// of a channel: where eight rows are an aligned run of slots a thread takes
+// whole pieces apart (four words of one lane, for all eight rows), else a row's
+// own codes are picked out of them; the codes meet in LDS as bytes and leave
+// row by row, 16 values of a block's scale at a time.  A slot outside the cache
+// reads as zeros.  Bound by HBM.
 template <int Q, int NB, typename T>
 __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
     using C = KvChunk<Q, NB>;
     constexpr int D = 32 * NB;
-    const int tid = threadIdx.x, head = blockIdx.y, g = tid & 3;
+    __shared__ int32_t sl[KV_ROWS];
+    __shared__ uint8_t codes_lds[KV_ROWS * D];
+    __shared__ uint16_t scales_lds[KV_ROWS * NB];
+    __shared__ uint64_t runs;
+    const int tid = threadIdx.x, head = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
     T *y = (T *)(is_v ? a.y[1] : a.y[0]);
-    const int64_t r = (int64_t)blockIdx.x * KV_ROWS + (tid >> 2);
-    if (!y || r >= a.n) return;
-    const int64_t s = a.slots[r];
-    const bool in = s >= 0 && s < a.c.slots;
-    const uint8_t *ck = chunk_of(a.c, in ? s : 0, head, C::BYTES) + (is_v ? C::HALF : 0);
-    const int key = (int)(s & 31);
-    y += (r * a.c.heads + head) * D;
-    // each value once: code · scale in fp32 (exact), rounded to the row's type
-    auto value = [&](int code, uint16_t d) { return in ? (float)code * (float)__builtin_bit_cast(_Float16, d) : 0.f; };
+    if (!y) return;
+    const int64_t r0 = (int64_t)blockIdx.x * KV_ROWS;
+    const int rows = (int)min((int64_t)KV_ROWS, a.n - r0);
+    y += (r0 * a.c.heads + head) * D;
+    const int64_t ld = (int64_t)a.c.heads * D;
+
     if (!is_v) {
-        const int t = (key >> 2) & 1, row = 4 * (key >> 3) + (key & 3);
+        const int g = tid & 3, r = tid >> 2;
+        if (r >= rows) return;
+        const int64_t s = a.slots[r0 + r];
+        const bool in = s >= 0 && s < a.c.slots;
+        const uint8_t *ck = chunk_of(a.c, in ? s : 0, head, C::BYTES);
+        const int key = (int)(s & 31), t = (key >> 2) & 1, row = 4 * (key >> 3) + (key & 3);
+        uint64_t w[NB];
+        if constexpr (NB % C::PER == 0) {
+#pragma unroll
+            for (int b = 0; b < NB; b += C::PER) load_piece<Q, NB>(ck, (t * NB + b) / C::PER, 16 * g + row, w + b);
+        } else {
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint8_t *at = ck + C::word(t * NB + b, 16 * g + row);
+                if constexpr (Q == 4) w[b] = *(const uint32_t *)at;
+                else w[b] = *(const uint64_t *)at;
+            }
+        }
+        float d[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) d[b] = (float)*(const _Float16 *)(ck + C::CODES + (b * 32 + key) * 2);
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const uint64_t w = load_word<Q>(ck + C::word(t * NB + b, 16 * g + row));
-            const uint16_t d = *(const uint16_t *)(ck + C::CODES + (b * 32 + key) * 2);
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = value(code_of<Q>(w, j), d);
-            T *o = y + 32 * b + 8 * g;
-            if constexpr (sizeof(T) == 2) {
-                h8 z;
-#pragma unroll
-                for (int j = 0; j < 8; j++) z[j] = (_Float16)v[j];
-                *(h8 *)o = z;
-            } else {
-                *(float4 *)o = make_float4(v[0], v[1], v[2], v[3]);
-                *(float4 *)(o + 4) = make_float4(v[4], v[5], v[6], v[7]);
-            }
+            for (int j = 0; j < 8; j++) v[j] = in ? (float)(int8_t)code_of<Q>(w[b], j) * d[b] : 0.f;
+            store8(y + r * ld + 32 * b + 8 * g, v);
         }
         return;
     }
+
+    if (tid < KV_ROWS) {
+        int32_t s = tid < rows ? a.slots[r0 + tid] : -1;
+        if (s < 0 || s >= a.c.slots) s = -1;
+        sl[tid] = s;
+        // (rows 0 .. 63 are one wave) bit r: rows r .. r + 8 are an aligned run
+        bool run = s >= 0 && (s & 7) == 0 && tid + 8 <= KV_ROWS;
 #pragma unroll
-    for (int w = 0; w < C::WORDS; w++) {
-        const uint16_t d = *(const uint16_t *)(ck + C::CODES + ((w >> 1) * 32 + key) * 2);
-        float v[4];
+        for (int m = 1; m < 8; m++) run = run & (__shfl(s, min(tid + m, KV_ROWS - 1), 64) == s + m);
+        const uint64_t b = __ballot(run);
+        if (tid == 0) runs = b;
+    }
+    __syncthreads();
+    const uint64_t starts = runs;
+    // whole runs: unit (row, piece, channel m of 16) where a run starts
+    for (int u = tid; u < KV_ROWS / 8 * C::PIECES * 16; u += 256) {
+        const int m = u & 15, p = (u >> 4) % C::PIECES;
+        uint64_t left = starts;
+        for (int k = (u >> 4) / C::PIECES; k > 0; k--) left &= left - 1;  // the k-th start
+        if (!left) continue;
+        const int r = __ffsll((unsigned long long)left) - 1, s = sl[r];
+        uint64_t w[C::PER];
+        load_piece<Q, NB>(chunk_of(a.c, s, head, C::BYTES) + C::HALF, p, 16 * ((s & 31) >> 3) + m, w);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            v[i] = value(code_of<Q>(load_word<Q>(ck + C::word(w, 16 * (key >> 3) + 4 * g + i)), key & 7), d);
-        T *o = y + 16 * w + 4 * g;
-        if constexpr (sizeof(T) == 2) {
-            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-            *(h4 *)o = h4{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3]};
-        } else {
-            *(float4 *)o = make_float4(v[0], v[1], v[2], v[3]);
+        for (int i = 0; i < C::PER; i++)
+            if (i < C::width(p)) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) codes_lds[(r + j) * D + 16 * (p * C::PER + i) + m] = (uint8_t)code_of<Q>(w[i], j);
+            }
+    }
+    // lone rows: thread 16r + m, its channels 16w + m
+    for (int u = tid; u < KV_ROWS * 16; u += 256) {
+        const int m = u & 15, r = u >> 4, s = sl[r];
+        const uint64_t before = starts & (r == 63 ? ~0ull : (2ull << r) - 1);  // runs that start at r or earlier
+        const bool covered = before && r - (63 - __clzll((long long)before)) < 8;
+        if (s < 0 || covered) continue;
+        const uint8_t *cv = chunk_of(a.c, s, head, C::BYTES) + C::HALF;
+#pragma unroll
+        for (int p = 0; p < C::PIECES; p++) {
+            uint64_t w[C::PER];
+            load_piece<Q, NB>(cv, p, 16 * ((s & 31) >> 3) + m, w);
+#pragma unroll
+            for (int i = 0; i < C::PER; i++)
+                if (i < C::width(p)) codes_lds[r * D + 16 * (p * C::PER + i) + m] = (uint8_t)code_of<Q>(w[i], s & 7);
         }
+    }
+    for (int u = tid; u < KV_ROWS * NB; u += 256) {
+        const int r = u / NB, b = u % NB, s = sl[r];
+        scales_lds[u] = s < 0 ? 0 : *(const uint16_t *)(chunk_of(a.c, s, head, C::BYTES) + C::HALF + C::CODES + (b * 32 + (s & 31)) * 2);
+    }
+    __syncthreads();
+    for (int u = tid; u < rows * (D / 8); u += 256) {
+        const int r = u / (D / 8), q = u % (D / 8);
+        const uint2 c = *(const uint2 *)(codes_lds + r * D + 8 * q);
+        const float d = (float)__builtin_bit_cast(_Float16, scales_lds[r * NB + (q >> 2)]);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = sl[r] < 0 ? 0.f : (float)(int8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3))) * d;
+        store8(y + r * ld + 8 * q, v);
     }
 }
 

@@ -106,12 +106,20 @@ __device__ __forceinline__ float sum_over_keys(float x) {
     return x + __shfl_xor(x, 32, 64);
 }
 
-// P·d of two neighbouring keys as an fp16 pair, each product rounded once.
-__device__ __forceinline__ uint32_t scaled_pair(float p0, float p1, uint32_t d) {
-    uint32_t r;
-    __asm__("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,1,0]\n\tv_fma_mixhi_f16 %0, %2, %3, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]"
-            : "=&v"(r) : "v"(p0), "v"(p1), "v"(d));
-    return r;
+// P·d of eight keys in fp16, each product rounded once.  (The compiler puts no
+// wait states around asm: one before it, behind the exponential that made p,
+// and two at its end, before the MFMA that reads the pairs.)
+__device__ __forceinline__ kv_u4 scaled_eight(const float *p, kv_u4 d) {
+    uint32_t r0, r1, r2, r3;
+#define S3E_KV_PAIR(R, P0, P1, D)                                        \
+    "v_fma_mixlo_f16 " R ", " P0 ", " D ", 0 op_sel_hi:[0,1,0]\n\t"      \
+    "v_fma_mixhi_f16 " R ", " P1 ", " D ", 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]\n\t"
+    __asm__("s_nop 0\n\t" S3E_KV_PAIR("%0", "%4", "%5", "%12") S3E_KV_PAIR("%1", "%6", "%7", "%13") S3E_KV_PAIR("%2", "%8", "%9", "%14")
+                S3E_KV_PAIR("%3", "%10", "%11", "%15") "s_nop 1"
+            : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+            : "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]), "v"(d[0]), "v"(d[1]), "v"(d[2]), "v"(d[3]));
+#undef S3E_KV_PAIR
+    return kv_u4{r0, r1, r2, r3};
 }
 
 // A mask over the fp16 pair of keys 2j, 2j + 1: zeros for those in `hidden`.
@@ -432,12 +440,12 @@ struct KvColumns {
                 for (int j = 0; j < 4; j++) d[j] &= keep_pair(h, j);
             }
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++) {
+                if constexpr (!F32) {
+                    p[n][0] = scaled_eight(t[n], d);
+                } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if constexpr (!F32) {
-                        p[n][0][j] = scaled_pair(t[n][2 * j], t[n][2 * j + 1], d[j]);
-                    } else {
+                    for (int j = 0; j < 4; j++) {
                         const kv_h2 dd = as_h2(d[j]);
                         float x = t[n][2 * j] * (float)dd[0], y = t[n][2 * j + 1] * (float)dd[1];
                         // one value for hi and for lo: folded into a mixed fma, hi alone would be rounded from the exact product
@@ -447,6 +455,7 @@ struct KvColumns {
                         p[n][PARTS - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
                     }
                 }
+            }
             if (NT > 1 && partly) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {

@@ -14,10 +14,10 @@
 // rounding but q's own.  V's scale varies along the summed dimension and goes
 // into the probabilities: P·d is rounded once, to fp16 (fp32 operands: kept as
 // a pair hi + lo, as is q, scaled by its row's power of two).  So that P·d
-// stays below fp16's largest and well above its smallest, a wave measures a
-// column's exponents from a reference: the column's largest score so far plus
-// the exponent of the largest scale of V so far; both are taken again, and the
-// accumulators scaled, when a score exceeds its by 8 or a scale exceeds its
+// stays below fp16's largest and well above its smallest, a column's exponents
+// are measured from a reference: its largest score so far plus the exponent of
+// the largest scale of V among the keys it has seen; both are taken again, and
+// the accumulators scaled, when a score exceeds its by 8 or a scale exceeds its
 // own (P·d ≤ 2^15 in between).
 #pragma once
 
@@ -127,6 +127,12 @@ __device__ __forceinline__ uint32_t keep_pair(uint32_t hidden, int j) {
     return (hidden >> 2 * j & 1 ? 0u : 0xffffu) | (hidden >> 2 * j & 2 ? 0u : 0xffff0000u);
 }
 
+// The larger of each of two 16-bit numbers.
+__device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
+    typedef uint16_t u2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, a), __builtin_bit_cast(u2, b)));
+}
+
 // s_waitcnt's field for at most n vector-memory operations under way.
 constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
@@ -212,7 +218,8 @@ struct KvColumns {
     kv_h8 qf[NT][NB][PARTS];
     kv_f4 acc[NT][W];
     float ref[NT], sum[NT];  // reference (log2) and this lane's part of the sum
-    int ed;                  // |scales of V so far| ≤ 2^ed
+    float room[NT];          // 15 − e, |scales of V of the keys seen so far| ≤ 2^e
+    uint32_t bound;          // fp16 bits of the least 2^e of the wave's columns that have seen a key
     const KvMagic M;
 
     // This lane's column of each tile: its query, head and limit (past the last
@@ -222,9 +229,10 @@ struct KvColumns {
         c0 = first;
         const int i_first = min(c0, k.ncols - 1) / k.G;
         see_all = a.causal ? min(k.len, k.len - k.nq + i_first + 1) : k.len;
-        ed = -24;
+        bound = 0x7fff;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
+            room[n] = 39.f;
             ref[n] = KV_NONE;
             sum[n] = 0.f;
 #pragma unroll
@@ -383,39 +391,52 @@ struct KvColumns {
             float x = fmaxf(fmaxf(t[n][0], t[n][1]), t[n][2]);
             x = fmaxf(fmaxf(x, t[n][3]), t[n][4]);
             mx[n] = fmaxf(fmaxf(x, t[n][5]), fmaxf(t[n][6], t[n][7])) * c1[n];
-            grow = grow || mx[n] > ref[n] + (float)(15 - ed);
+            grow = grow || mx[n] > ref[n] + room[n];
         }
-        const uint32_t bound = (uint32_t)(ed >= -14 ? (ed + 15) << 10 : 1 << (ed + 24));  // fp16 bits of 2^ed
 #pragma unroll
         for (int i = 0; i < VD; i++) grow = grow || (vds[i] & 0x7fffu) > bound || ((vds[i] >> 16) & 0x7fffu) > bound;
         if (__builtin_amdgcn_ballot_w64(grow)) {
-            // V's largest scale among keys of the sequence; not those that are no numbers
-            uint32_t dm = 0;
+            // the largest scales of V by key; not those that are no numbers
+            uint32_t dk[4] = {0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < VD; i++) {
-                const int k2 = 32 * g + 2 * ((lane + 64 * i) & 15);
-                const uint32_t lo = vds[i] & 0x7fffu, hi = (vds[i] >> 16) & 0x7fffu;
-                if (have && k2 < len && lo < 0x7c00u) dm = max(dm, lo);
-                if (have && k2 + 1 < len && hi < 0x7c00u) dm = max(dm, hi);
+            for (int b = 0; b < NB; b++) {
+                const kv_u4 d = vscale(b);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t x = d[j] & 0x7fff7fffu;
+                    dk[j] = max_u16(dk[j], x & ~(((x + 0x04000400u) >> 15 & 0x00010001u) * 0xffffu));
+                }
             }
-#pragma unroll
-            for (int x = 1; x < 64; x *= 2) dm = max(dm, (uint32_t)__shfl_xor((int)dm, x, 64));
-            // 2^en ≥ every scale: one above the exponent, or of a subnormal its bit length − 24
-            const int en = dm >= 0x400u ? (int)(dm >> 10) - 14 : 8 - (dm ? __builtin_clz(dm) : 32);
-            const int ed_n = max(ed, __builtin_amdgcn_readfirstlane(en));
+            uint32_t low = 0x7fff;
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                // the reference is the largest score + ed − 7
-                const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (float)(ed - 7);
-                const float top = fmaxf(best, max_over_keys(mx[n]));
-                const float ref_n = top <= KV_NONE ? KV_NONE : top + (float)(ed_n - 7);
+                // of those of the keys that the column sees
+                uint32_t dm = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) dm = max_u16(dm, dk[j] & (special ? keep_pair(hidden[n], j) : ~0u));
+                dm = max(dm & 0xffffu, dm >> 16);
+                dm = max(dm, (uint32_t)__shfl_xor((int)dm, 16, 64));
+                dm = max(dm, (uint32_t)__shfl_xor((int)dm, 32, 64));
+                // 2^e ≥ every scale: one above the exponent, or of a subnormal its bit length − 24
+                const int e = dm >= 0x400u ? (int)(dm >> 10) - 14 : 8 - (dm ? __builtin_clz(dm) : 32);
+                // the reference is the largest score + e − 7 (of a column that
+                // outgrew its own: what others see changes nothing of it)
+                const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (8.f - room[n]), up = max_over_keys(mx[n]);
+                const float top = fmaxf(best, up);
+                const bool mine = up > ref[n] + room[n] || (float)(15 - e) < room[n];
+                room[n] = fminf(room[n], (float)(15 - e));
+                const float ref_n = !mine ? ref[n] : (top <= KV_NONE ? KV_NONE : top + (8.f - room[n]));
                 const float alpha = ref_n == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - ref_n);
                 ref[n] = ref_n;
                 sum[n] *= alpha;
 #pragma unroll
                 for (int w = 0; w < W; w++) acc[n][w] *= alpha;
+                const int ed = 15 - (int)room[n];
+                if (ref_n != KV_NONE) low = min(low, ed >= -14 ? (uint32_t)(ed + 15) << 10 : 1u << (ed + 24));
             }
-            ed = ed_n;
+#pragma unroll
+            for (int x = 1; x < 16; x *= 2) low = min(low, (uint32_t)__shfl_xor((int)low, x, 64));
+            bound = __builtin_amdgcn_readfirstlane(low);
         }
 
         // ---- probabilities, in units of the reference

@@ -396,6 +396,33 @@ def test_hidden_keys_reach_nothing(ctx, t, io):
 
 
 @pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("t", [ref.Q4_0, ref.Q8_0])
+@pytest.mark.parametrize("nq", [3, 40])
+@pytest.mark.parametrize("masked", [False, True])
+def test_large_hidden_values_change_nothing(ctx, t, io, nq, masked):
+    # keys that a row does not see (later ones, or masked ones) with values near the largest a cache holds, among
+    # small ones: the row's bits are those beside small keys.  nq: one or more column tiles
+    heads, nh, D, page, kv = 1, 2, 64, 64, 120
+    x = Batch(ctx, t, io, heads, nh, D, page, [(nq, kv)], seed=21, mask=masked, causal=not masked)
+    hide = np.arange(kv) >= kv - nq // 2 if not masked else np.arange(kv) % 9 == 4
+    rows = np.arange(nq) < nq - nq // 2 if not masked else np.ones(nq, bool)
+    if masked:
+        x.mask[:, :kv] = np.where(hide, -np.inf, 0)
+        x.md.upload(x.mask)
+    table = x.arrays[2].download(np.int32, (1, -(-kv // page)))
+    slots = ctx.to_device(np.array([table[0, j // page] * page + j % page for j in range(kv)], np.int32))
+    nb = (heads * D, D)
+    outs = []
+    for large in (1e-3, 1e5):
+        k, v = x.k * 1.0, x.v * 1e-3
+        v[hide] *= large / 1e-3
+        ctx.kv_write(x.c, s3e.TYPE_F32, ctx.to_device(k.astype(np.float32)), nb, ctx.to_device(v.astype(np.float32)), nb, slots, kv)
+        outs.append(x.run()[rows])
+    assert np.isfinite(outs[0]).all() and np.abs(outs[0]).max() > 0
+    assert np.array_equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
 def test_values_that_are_no_numbers_come_through(ctx, io):
     x = Batch(ctx, ref.Q8_0, io, 1, 1, 64, 64, [(1, 90), (1, 40)], seed=2)
     x.v[3, 0, 0] = np.nan    # the first block of key 3 of the first sequence

@@ -305,12 +305,14 @@ int s3e_kv_cache_bytes(const s3e_kv_cache *c, size_t *bytes);
  * holds an infinity or a NaN reads back as NaN; a scale past fp16 is infinite.
  * A row whose slot is negative or past the cache is left out; the slots of the
  * others are distinct (of a slot given twice the contents are unspecified).
- * Other slots keep their bytes.  Asynchronous on the context's stream; allocates nothing. */
+ * Other slots keep their bytes.  k, v and slots lie outside the cache's memory;
+ * n is at most 2^29.  Asynchronous on the context's stream; allocates nothing. */
 int s3e_kv_write(s3e_ctx *ctx, const s3e_kv_cache *c, int type, const void *k, const int64_t k_nb[2],
                  const void *v, const int64_t v_nb[2], const int32_t *slots, int64_t n);
 /* Read n slots back (ggml_get_rows): k and v receive [n][n_heads][D] values of
  * `type` (16-byte aligned), each scale · code rounded to it once; either may be
- * NULL.  A slot that is negative or past the cache reads as zeros.
+ * NULL.  A slot that is negative or past the cache reads as zeros.  k and v
+ * overlap neither each other nor the cache or the slots; n is at most 2^29.
  * Asynchronous; allocates nothing. */
 int s3e_kv_read(s3e_ctx *ctx, const s3e_kv_cache *c, const int32_t *slots, int64_t n, int type, void *k, void *v);
 
@@ -343,9 +345,10 @@ int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t 
  * the cache does not have (its keys are hidden).  A row that sees no key is
  * zero.  Rows outside every sequence are left as they are, and so are rows
  * of a sequence past max_q; keys past max_kv are not seen.  o may be q itself
- * (same type, contiguous) but must not overlap it otherwise, nor the cache.
+ * (same type, contiguous) but overlaps nothing else that the call reads.
  * ws: device, 16-byte aligned, ws_bytes of it, this call's own until it has
- * run; with it the call allocates nothing and can be captured.  Asynchronous. */
+ * run and outside all of the above; with it the call allocates nothing and can
+ * be captured.  Asynchronous. */
 int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_batch *b, int type, const void *q,
                 const int64_t q_nb[2], int64_t nh, float scale, int causal, const uint16_t *mask, int64_t mask_ld,
                 void *o, void *ws, size_t ws_bytes);

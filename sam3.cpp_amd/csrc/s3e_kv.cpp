@@ -59,17 +59,27 @@ KvCache on_device(const s3e_kv_cache *c) {
     return k;
 }
 
+// Rows of a call: a grid's threads along one dimension stay below 2^32.
+constexpr int64_t KV_MAX_ROWS = 1 << 29;
+
 int check_type(const char *fn, int type) {
     if (type != S3E_TYPE_F32 && type != S3E_TYPE_F16) KV_REFUSE(S3E_ERR_UNSUPPORTED, "%s: rows of type %d (F32 or F16)", fn, type);
     return S3E_OK;
 }
 
-// Rows by element strides: whether they lie on their type's alignment, and
-// whether 16-byte loads may read them.
-int check_rows(const char *fn, const char *what, const void *p, const int64_t nb[2], int64_t esize, int *vec) {
+// n rows of `heads` times D values by element strides: whether they lie on their
+// type's alignment, whether 16-byte loads may read them, and the bytes from the
+// first to the last.
+int check_rows(const char *fn, const char *what, const void *p, const int64_t nb[2], int64_t n, int64_t heads, int64_t D,
+               int64_t esize, int *vec, size_t *bytes) {
     if (nb[0] < 0 || nb[1] < 0) KV_REFUSE(S3E_ERR_INVALID, "%s: a negative stride of %s", fn, what);
     if ((uintptr_t)p % (uintptr_t)esize != 0) KV_REFUSE(S3E_ERR_INVALID, "%s: %s is not aligned to its type", fn, what);
-    *vec = (uintptr_t)p % 16 == 0 && nb[0] * esize % 16 == 0 && nb[1] * esize % 16 == 0;
+    const __int128 span = n <= 0 ? 0 : ((__int128)(n - 1) * nb[0] + (__int128)(heads - 1) * nb[1] + D) * esize;
+    if (span > INT64_MAX) KV_REFUSE(S3E_ERR_INVALID, "%s: strides of %s past any memory", fn, what);
+    // (a stride that no row takes says nothing)
+    const bool rows_vec = n <= 1 || nb[0] * esize % 16 == 0, heads_vec = heads <= 1 || nb[1] * esize % 16 == 0;
+    *vec = (uintptr_t)p % 16 == 0 && rows_vec && heads_vec;
+    *bytes = (size_t)span;
     return S3E_OK;
 }
 
@@ -98,7 +108,7 @@ constexpr int64_t KV_MIN_KEYS = 256;
 // alone, so that a captured call is the same for any lengths.
 void plan(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, bool f32, KvAttnArgs &a) {
     a.n_seq = (int)b->n_seq;
-    kv_attn_columns(a, c->head_dim, f32, b->max_q * (nh / c->n_heads));
+    kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * (nh / c->n_heads));
     const int64_t wgs = b->n_seq * c->n_heads * a.ctiles;
     int64_t ns = a.tile ? a.goal / wgs : (a.goal + wgs - 1) / wgs;
     ns = std::max<int64_t>(1, std::min(ns, (b->max_kv + KV_MIN_KEYS - 1) / KV_MIN_KEYS));
@@ -126,13 +136,19 @@ extern "C" int s3e_kv_write(s3e_ctx *ctx, const s3e_kv_cache *c, int type, const
     int rc = check_cache(fn, c, true);
     if (rc == S3E_OK) rc = check_type(fn, type);
     if (rc != S3E_OK) return rc;
-    if (n < 0 || n > INT32_MAX) { set_error("%s: %lld rows", fn, (long long)n); return S3E_ERR_INVALID; }
+    if (n < 0 || n > KV_MAX_ROWS) { set_error("%s: %lld rows", fn, (long long)n); return S3E_ERR_INVALID; }
     KvWriteArgs a;
     const int64_t esize = type == S3E_TYPE_F32 ? 4 : 2;
-    rc = check_rows(fn, "k", k, k_nb, esize, &a.vec[0]);
-    if (rc == S3E_OK) rc = check_rows(fn, "v", v, v_nb, esize, &a.vec[1]);
+    size_t k_bytes = 0, v_bytes = 0;
+    rc = check_rows(fn, "k", k, k_nb, n, c->n_heads, c->head_dim, esize, &a.vec[0], &k_bytes);
+    if (rc == S3E_OK) rc = check_rows(fn, "v", v, v_nb, n, c->n_heads, c->head_dim, esize, &a.vec[1], &v_bytes);
     if (rc != S3E_OK) return rc;
     if (n == 0) return S3E_OK;
+    const size_t cb = cache_bytes(c);
+    if (meets(k, k_bytes, c->data, cb) || meets(v, v_bytes, c->data, cb) || meets(slots, (size_t)n * 4, c->data, cb)) {
+        set_error("%s: k, v or slots overlap the cache", fn);
+        return S3E_ERR_INVALID;
+    }
     a.x[0] = k, a.x[1] = v;
     a.st[0] = k_nb[0], a.sh[0] = k_nb[1];
     a.st[1] = v_nb[0], a.sh[1] = v_nb[1];
@@ -151,9 +167,16 @@ extern "C" int s3e_kv_read(s3e_ctx *ctx, const s3e_kv_cache *c, const int32_t *s
     int rc = check_cache(fn, c, true);
     if (rc == S3E_OK) rc = check_type(fn, type);
     if (rc != S3E_OK) return rc;
-    if (n < 0 || n > INT32_MAX) { set_error("%s: %lld rows", fn, (long long)n); return S3E_ERR_INVALID; }
+    if (n < 0 || n > KV_MAX_ROWS) { set_error("%s: %lld rows", fn, (long long)n); return S3E_ERR_INVALID; }
     if ((uintptr_t)k % 16 != 0 || (uintptr_t)v % 16 != 0) { set_error("%s: k and v must be 16-byte aligned", fn); return S3E_ERR_INVALID; }
     if (n == 0) return S3E_OK;
+    const size_t cb = cache_bytes(c), yb = (size_t)n * c->n_heads * c->head_dim * (type == S3E_TYPE_F32 ? 4 : 2);
+    const size_t kb = k ? yb : 0, vb = v ? yb : 0;
+    if (meets(k, kb, v, vb) || meets(k, kb, c->data, cb) || meets(v, vb, c->data, cb) || meets(k, kb, slots, (size_t)n * 4) ||
+        meets(v, vb, slots, (size_t)n * 4)) {
+        set_error("%s: k and v overlap each other, the cache or the slots", fn);
+        return S3E_ERR_INVALID;
+    }
     KvReadArgs a;
     a.y[0] = k, a.y[1] = v;
     a.slots = slots;
@@ -193,7 +216,9 @@ extern "C" int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_bat
     const bool f32 = type == S3E_TYPE_F32;
     const int64_t esize = f32 ? 4 : 2;
     KvAttnArgs a;
-    rc = check_rows(fn, "q", q, q_nb, esize, &a.q_vec);
+    const int64_t D = c->head_dim;
+    size_t qb = 0;
+    rc = check_rows(fn, "q", q, q_nb, b->n_tokens, nh, D, esize, &a.q_vec, &qb);
     if (rc != S3E_OK) return rc;
     if ((uintptr_t)o % 16 != 0) { set_error("%s: o must be 16-byte aligned", fn); return S3E_ERR_INVALID; }
     if (mask && (mask_ld < b->max_kv || (uintptr_t)mask % 2 != 0)) {
@@ -202,12 +227,17 @@ extern "C" int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_bat
     }
     if (b->n_seq == 0 || b->n_tokens == 0 || b->max_q == 0) return S3E_OK;
     if (!b->q_start || !b->kv_len || !b->pages) { set_error("%s: the batch lacks an array", fn); return S3E_ERR_INVALID; }
-    const int64_t D = c->head_dim;
     const size_t ob = (size_t)(b->n_tokens * nh * D * esize);
-    const size_t qb = (size_t)(((b->n_tokens - 1) * q_nb[0] + (nh - 1) * q_nb[1] + D) * esize);
+    const __int128 mask_span = mask ? ((__int128)(b->n_tokens - 1) * mask_ld + b->max_kv) * 2 : 0;
+    if (mask_span > INT64_MAX) { set_error("%s: mask rows of %lld past any memory", fn, (long long)mask_ld); return S3E_ERR_INVALID; }
     const bool in_place = o == q && q_nb[0] == nh * D && (nh == 1 || q_nb[1] == D);
     if (!in_place && meets(o, ob, q, qb)) { set_error("%s: o overlaps q", fn); return S3E_ERR_INVALID; }
     if (meets(o, ob, c->data, cache_bytes(c))) { set_error("%s: o overlaps the cache", fn); return S3E_ERR_INVALID; }
+    // what every work-group reads stays as it is
+    struct { const void *p; size_t n; } read[] = {{mask, (size_t)mask_span}, {b->q_start, (size_t)(b->n_seq + 1) * 4},
+                                                  {b->kv_len, (size_t)b->n_seq * 4}, {b->pages, (size_t)(b->n_seq * b->pages_ld) * 4}};
+    for (const auto &r : read)
+        if (meets(o, ob, r.p, r.n)) { set_error("%s: o overlaps the mask or an array of the batch", fn); return S3E_ERR_INVALID; }
     plan(c, b, nh, f32, a);
     const size_t need = partial_bytes(c, b, nh, a);
     if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 16 != 0)) {
@@ -218,6 +248,8 @@ extern "C" int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_bat
         set_error("%s: the workspace overlaps q, o or the cache", fn);
         return S3E_ERR_INVALID;
     }
+    for (const auto &r : read)
+        if (meets(ws, need, r.p, r.n)) { set_error("%s: the workspace overlaps the mask or an array of the batch", fn); return S3E_ERR_INVALID; }
     a.c = on_device(c);
     a.q = q;
     a.q_st = q_nb[0], a.q_sh = q_nb[1];

@@ -116,6 +116,47 @@ def test_bad_attention_arguments():
     assert attn(type_=s3e.TYPE_Q8_0) == UNSUPPORTED
 
 
+def test_overlaps_are_refused():
+    c = cache()
+    nb = s3e.kv_cache_bytes(c)
+    far = FAKE + (1 << 30)
+    ok = dict(k=far, v=far, slots=far + (1 << 20))  # (k and v may be the same rows)
+    # the last row of k or v, or the slots, run into the cache: three rows of two heads of 64 floats
+    for over in (dict(k=FAKE - 1532), dict(v=FAKE + nb - 4), dict(slots=FAKE - 8)):
+        assert write(c, **{**ok, **over}) == INVALID, over
+        assert b"overlap" in s3e.LIB.s3e_last_error()
+    ok = dict(k=far, v=far + 3 * 512, slots=far + (1 << 20))
+    for over in (dict(v=far + 3 * 512 - 16), dict(k=FAKE - 1520), dict(v=FAKE + nb - 16), dict(slots=far + 1024), dict(k=None, slots=far + 3 * 512)):
+        assert read(c, **{**ok, **over}) == INVALID, over
+        assert b"overlap" in s3e.LIB.s3e_last_error()
+    # the output of attention: six rows of four heads of 64 floats
+    ob = 6 * 4 * 64 * 4
+    for over in (dict(mask=O + ob - 2, mask_ld=256), dict(mask=O - 16, mask_ld=200)):
+        assert attn(**over) == INVALID, over
+        assert b"overlap" in s3e.LIB.s3e_last_error()
+    for name in ("q_start", "kv_len", "pages"):
+        assert attn(b=batch(**{name: Buf(O + ob - 4)})) == INVALID, name
+        assert b"overlap" in s3e.LIB.s3e_last_error()
+    # the workspace
+    b = dict(n_seq=1, n_tokens=1, max_q=1, max_kv=100000, pages_ld=2000)
+    c = cache(n_pages=2000)
+    far = FAKE + (1 << 36)
+    for name in ("q_start", "kv_len", "pages"):
+        assert attn(c, batch(**b, **{name: Buf(WS + 64)}), o=far) == INVALID, name
+        assert b"overlap" in s3e.LIB.s3e_last_error()
+    assert attn(c, batch(**b), o=far, mask=WS + 64, mask_ld=100000) == INVALID
+    assert b"overlap" in s3e.LIB.s3e_last_error()
+
+
+def test_strides_past_any_memory_are_refused():
+    far = FAKE + (1 << 30)
+    for nb in ((1 << 62, 64), (128, 1 << 62), (1 << 60, 64)):
+        assert write(cache(), k=far, v=far, k_nb=nb) == INVALID and b"strides" in s3e.LIB.s3e_last_error(), nb
+        assert attn(q_nb=nb) == INVALID and b"strides" in s3e.LIB.s3e_last_error(), nb
+    assert attn(mask=far, mask_ld=1 << 61) == INVALID and b"mask" in s3e.LIB.s3e_last_error()
+    assert write(cache(), n=(1 << 29) + 1) == INVALID and read(cache(), n=(1 << 29) + 1) == INVALID
+
+
 def test_workspace_is_checked():
     # one long sequence: its keys go in ranges, whose partial results need memory
     b = batch(n_seq=1, n_tokens=1, max_q=1, max_kv=100000, pages_ld=2000)

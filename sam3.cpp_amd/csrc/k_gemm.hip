@@ -1322,9 +1322,10 @@ __global__ __launch_bounds__(256, 3) void k_gemm_f6(GemmParams p) {
 }
 
 // y = Σ_k part[k] (+ bias) for EPI_F32, y += Σ_k part[k] (+ bias) for
-// EPI_RESID (resid is y), y = act(Σ_k part[k] (+ bias)) (+ resid) for
+// EPI_RESID (resid not null), y = act(Σ_k part[k] (+ bias)) (+ resid) for
 // EPI_FUSED, the ranges summed in order (the result does not depend on the
 // schedule).  One thread per 4 consecutive outputs of a row.
+template <bool FUSED>
 __global__ __launch_bounds__(256) void k_gemm_reduce(const float *__restrict__ part, int ks, int M, int N,
                                                      const float *__restrict__ bias, float *y, int64_t ldy,
                                                      const float *resid, int act) {
@@ -1348,13 +1349,25 @@ __global__ __launch_bounds__(256) void k_gemm_reduce(const float *__restrict__ p
         v.z = __fadd_rn(v.z, bias[c + 2]);
         v.w = __fadd_rn(v.w, bias[c + 3]);
     }
-    if (act) v = make_float4(act_f32(act, v.x), act_f32(act, v.y), act_f32(act, v.z), act_f32(act, v.w));
+    if constexpr (FUSED) v = make_float4(act_f32(act, v.x), act_f32(act, v.y), act_f32(act, v.z), act_f32(act, v.w));
     float4 *o = (float4 *)(y + (int64_t)r * ldy + c);
     if (resid) {
-        const float4 x = *(const float4 *)(resid + (int64_t)r * ldy + c);
+        const float4 x = FUSED ? *(const float4 *)(resid + (int64_t)r * ldy + c) : *o;
         v = make_float4(__fadd_rn(x.x, v.x), __fadd_rn(x.y, v.y), __fadd_rn(x.z, v.z), __fadd_rn(x.w, v.w));
     }
     *o = v;
+}
+
+hipError_t launch_reduce(const GemmParams &p, Epi epi, hipStream_t st) {
+    const EpiArgs &e = p.e;
+    const dim3 grid((unsigned)(((int64_t)p.M * (p.N / 4) + 255) / 256));
+    if (epi == EPI_FUSED)
+        hipLaunchKernelGGL(k_gemm_reduce<true>, grid, dim3(256), 0, st, p.part, p.ksplit, p.M, p.N, e.bias, e.y, e.ldy,
+                           e.resid, e.act);
+    else
+        hipLaunchKernelGGL(k_gemm_reduce<false>, grid, dim3(256), 0, st, p.part, p.ksplit, p.M, p.N, e.bias, e.y, e.ldy,
+                           epi == EPI_RESID ? e.y : nullptr, 0);
+    return hipGetLastError();
 }
 
 template <int WK, int EPI, int BM, int WAVES, int RING = 0>
@@ -1569,15 +1582,7 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
             default: return hipErrorInvalidValue;
         }
         hipError_t e = hipGetLastError();
-        if (e == hipSuccess && p.ksplit > 1) {
-            const int64_t n = M * (w.N / 4);
-            hipLaunchKernelGGL(k_gemm_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p.part, p.ksplit,
-                               (int)M, (int)w.N, ea.bias, ea.y, ea.ldy,
-                               epi == EPI_RESID ? ea.y : (epi == EPI_FUSED ? ea.resid : nullptr),
-                               epi == EPI_FUSED ? ea.act : 0);
-            e = hipGetLastError();
-        }
-        return e;
+        return e == hipSuccess && p.ksplit > 1 ? launch_reduce(p, epi, st) : e;
     }
     // 64-row tiles: two or three work-groups share a CU, so one work-group's
     // epilogue overlaps another's main loop; with 128-row tiles (one per CU)
@@ -1592,15 +1597,7 @@ hipError_t launch_gemm(const Weight &w, const Act &a, int64_t M, Epi epi, const 
         case WK_F16X3: e = dispatch_waves<WK_F16X3>(epi, p, st); break;
         default: return hipErrorInvalidValue;
     }
-    if (e == hipSuccess && p.ksplit > 1) {
-        const int64_t n = M * (w.N / 4);
-        hipLaunchKernelGGL(k_gemm_reduce, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p.part, p.ksplit,
-                           (int)M, (int)w.N, ea.bias, ea.y, ea.ldy,
-                               epi == EPI_RESID ? ea.y : (epi == EPI_FUSED ? ea.resid : nullptr),
-                               epi == EPI_FUSED ? ea.act : 0);
-        e = hipGetLastError();
-    }
-    return e;
+    return e == hipSuccess && p.ksplit > 1 ? launch_reduce(p, epi, st) : e;
 }
 
 }  // namespace s3e

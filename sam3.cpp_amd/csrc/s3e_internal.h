@@ -181,12 +181,14 @@ struct EpiArgs {
     float *ws = nullptr;
     int64_t ws_cap = 0;
     Act out;                     // EPI_GELU
-    // EPI_FUSED: an s3e_act, and rows of ldy to add (may be y) or null
-    int act = 0;
-    const float *resid = nullptr;
-    // EPI_POS
-    const float *pos = nullptr;  // [pg][pg][E]
-    int pos_grid = 0;
+    union {
+        const float *pos = nullptr;  // EPI_POS: [pg][pg][E]
+        const float *resid;          // EPI_FUSED: rows of ldy to add (may be y) or null
+    };
+    union {
+        int pos_grid = 0;  // EPI_POS
+        int act;           // EPI_FUSED: an s3e_act
+    };
     // geometry shared by EPI_POS and EPI_QKV
     int grid = 0;                // tokens per side
     int window = 0;              // window side (== grid for global attention)

@@ -213,7 +213,7 @@ struct KvColumns {
     static constexpr int VD = (NB * 16 + 63) / 64;
 
     int c0, see_all;
-    int lim[NT], tok[NT], head[NT];
+    int tok[NT];
     float cs[NT];            // a score's units of log2
     kv_h8 qf[NT][NB][PARTS];
     kv_f4 acc[NT][W];
@@ -239,9 +239,7 @@ struct KvColumns {
             for (int w = 0; w < W; w++) acc[n][w] = kv_f4{0.f, 0.f, 0.f, 0.f};
             const int c = min(c0 + 16 * n + col, k.ncols - 1), i = c / k.G;
             tok[n] = k.q0 + i;
-            head[n] = k.kvh * k.G + (c - i * k.G);
-            lim[n] = a.causal ? min(k.len, k.len - k.nq + i + 1) : k.len;
-            const int64_t at = tok[n] * a.q_st + head[n] * a.q_sh + 8 * ka;
+            const int64_t at = tok[n] * a.q_st + (k.kvh * k.G + (c - i * k.G)) * a.q_sh + 8 * ka;
             if constexpr (!F32) {
                 cs[n] = a.scale;
                 const _Float16 *q = (const _Float16 *)a.q + at;
@@ -298,7 +296,7 @@ struct KvColumns {
     // the scales of this lane's eight keys, vbits(i) dwords of V's scales, of
     // which each of the chunk's NB · 16 is some lane's.
     template <typename KW, typename KS, typename VW, typename VS, typename VB>
-    __device__ __forceinline__ void chunk(const KvAttnArgs &a, int len, int g, bool have, int lane, KW kword, KS kscale, VW vword,
+    __device__ __forceinline__ void chunk(const KvAttnArgs &a, const KvTask &k, int g, bool have, int lane, KW kword, KS kscale, VW vword,
                                           VS vscale, VB vbits) {
         // ---- Sᵀ = K·Qᵀ, times K's scales: the next block's words are made
         // between a block's MFMAs and their use.  (The scheduling barriers keep
@@ -350,16 +348,17 @@ struct KvColumns {
                         for (int j = 0; j < 8; j++) mv[j] = (float)x[j];
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 8; j++) mv[j] = (float)mp[min(j, len - 1 - key0)];  // (all at once: past the end any value does)
+                        for (int j = 0; j < 8; j++) mv[j] = (float)mp[min(j, k.len - 1 - key0)];  // (all at once: past the end any value does)
                     }
 #pragma unroll
                     for (int j = 0; j < 8; j++)
                         t[n][j] = mv[j] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[j], 1.4426950408889634f, t[n][j] * cs[n]);
                 }
                 hidden[n] = 0;
+                const int lim = a.causal ? min(k.len, k.len - k.nq + tok[n] - k.q0 + 1) : k.len;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    if (!have || key0 + j >= lim[n]) t[n][j] = -INFINITY;
+                    if (!have || key0 + j >= lim) t[n][j] = -INFINITY;
                     hidden[n] |= t[n][j] == -INFINITY ? 1u << j : 0u;
                 }
             }
@@ -534,7 +533,8 @@ struct KvColumns {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             if (c0 + 16 * n + col >= k.ncols) continue;
-            const int64_t row = (int64_t)tok[n] * a.nh + head[n];
+            // (tok = q0 + c / G, head = kvh·G + c % G)
+            const int64_t row = (int64_t)tok[n] * a.nh + k.kvh * k.G + (c0 + 16 * n + col - (tok[n] - k.q0) * k.G);
             if (a.nsplit > 1) {
                 const int64_t at = (int64_t)k.split * a.n_tokens * a.nh + row;
                 float *o = a.part_o + at * D + 4 * ka;
@@ -624,7 +624,7 @@ __global__ __launch_bounds__(64 * KV_WAVES, kv_waves(NB, NT)) void k_kv_attn(KvA
             KvHalf<Q, NB> K, V;
             K.load(kh, lane);
             cols.chunk(
-                a, k.len, g, have, lane, [&](int i) { return K.word(i, cols.M); },
+                a, k, g, have, lane, [&](int i) { return K.word(i, cols.M); },
                 [&](int b) { return scales_of<Q, NB>(kh, b, ka); },
                 [&](int i) {
                     if (i == 0) V.load(vh, lane);
@@ -674,35 +674,41 @@ constexpr int kv_tile_waves(int NB, bool F32) { return NB == 8 && !F32 ? 12 : 8;
 constexpr int kv_tile_nt(int NB, bool F32) { return F32 ? (NB <= 2 ? 2 : 1) : (NB == 8 ? 1 : 2); }
 constexpr int kv_tile_fill(int NB, bool F32) { return F32 ? 2 : (NB <= 2 ? 4 : (NB == 8 ? 3 : 2)); }
 constexpr int kv_tile_streams(int NB) { return NB == 8 ? 1 : 2; }
+constexpr int kv_tile_chunks(int NB) { return NB <= 2 ? 2 : 1; }
 constexpr int kv_tile_cols(int NB, bool F32) { return 16 * kv_tile_nt(NB, F32) * kv_tile_waves(NB, F32) / kv_tile_streams(NB); }
 
 template <int Q, int NB, bool F32>
 __global__ __launch_bounds__(64 * kv_tile_waves(NB, F32), kv_tile_fill(NB, F32)) void k_kv_attn_tile(KvAttnArgs a) {
     using C = KvChunk<Q, NB>;
-    constexpr int NT = kv_tile_nt(NB, F32), KS = kv_tile_streams(NB), CG = kv_tile_waves(NB, F32) / KS;
+    constexpr int NT = kv_tile_nt(NB, F32), KS = kv_tile_streams(NB), CG = kv_tile_waves(NB, F32) / KS, CPT = kv_tile_chunks(NB);
     using Cols = KvColumns<NB, F32, NT, (NB > 4 || (!F32 && NB <= 2))>;
     constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
-    constexpr int W = Cols::W, BUFS = 2 * KS * BUF, JOIN = KS > 1 ? CG * NT * (W * 1024 + 512) : 0;
+    constexpr int W = Cols::W, BUFS = 2 * KS * CPT * BUF, JOIN = KS > 1 ? CG * NT * (W * 1024 + 512) : 0;
     __shared__ __attribute__((aligned(16))) uint8_t smem[BUFS > JOIN ? BUFS : JOIN];
 
     const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ks = wave / CG, cg = wave % CG, st = tid % (64 * CG);  // stream, column group, thread of the stream
+    const int ks = wave / CG, cg = wave % CG;  // stream, column group
     int s;
     const KvTask k = kv_task<kv_tile_cols(NB, F32)>(a, s);
     if (!k.some) return;
     const KvPlaces places(a, s, k.kvh, C::BYTES);
 
-    // pieces of K and V this wave converts, and the scales (16 bytes a thread)
-    constexpr int PW = (2 * C::PIECES + CG - 1) / CG;
-    static_assert(8 * NB <= 64 * CG, "a thread for every 16 bytes of scales");
+    // pieces of K and V this wave converts; wave c of a stream takes chunk c's scales
+    constexpr int P2 = 2 * C::PIECES, PW = (CPT * P2 + CG - 1) / CG, S2 = 8 * NB;
+    static_assert(S2 <= 64 && CPT <= CG && CPT <= 2, "a wave for the scales of each chunk");
     uint4 raw[PW], rawd;
-    auto fetch = [&](const uint8_t *p) {
+    const int g_end = (k.k_end + 31) >> 5;
+    // chunks g .. g + CPT, as far as there are any; `have` their pages
+    auto fetch = [&](int g, bool *have) {
+        const uint8_t *p[CPT];
+#pragma unroll
+        for (int c = 0; c < CPT; c++) p[c] = places.at(CPT > 1 ? min(g + c, g_end - 1) : g, have[c]);
 #pragma unroll
         for (int i = 0; i < PW; i++) {
             const int u = cg + i * CG, pi = u % C::PIECES;
-            if (u >= 2 * C::PIECES) continue;
-            const uint8_t *q = p + (u / C::PIECES) * C::HALF + pi * 1024 + lane * (C::width(pi) * Q);
+            if (u >= CPT * P2) continue;
+            const uint8_t *q = p[CPT > 1 && u >= P2 ? 1 : 0] + (u / C::PIECES % 2) * C::HALF + pi * 1024 + lane * (C::width(pi) * Q);
             if (C::width(pi) == C::PER) {
                 raw[i] = gload16(q);
             } else {
@@ -710,15 +716,16 @@ __global__ __launch_bounds__(64 * kv_tile_waves(NB, F32), kv_tile_fill(NB, F32))
                 raw[i] = make_uint4(x.x, x.y, 0, 0);
             }
         }
-        if (st < 8 * NB) rawd = gload16(p + C::CODES + (st < 4 * NB ? st * 16 : C::HALF + (st - 4 * NB) * 16));
+        if (cg < CPT && lane < S2)
+            rawd = gload16(p[CPT > 1 && cg ? 1 : 0] + C::CODES + (lane < 4 * NB ? lane * 16 : C::HALF + (lane - 4 * NB) * 16));
     };
     const KvMagic M;
     auto convert = [&](uint8_t *buf) {
 #pragma unroll
         for (int i = 0; i < PW; i++) {
             const int u = cg + i * CG, pi = u % C::PIECES;
-            if (u >= 2 * C::PIECES) continue;
-            uint8_t *o = buf + (u / C::PIECES) * HALF + pi * (C::PER * 1024) + lane * 16;
+            if (u >= CPT * P2) continue;
+            uint8_t *o = buf + (CPT > 1 && u >= P2 ? BUF : 0) + (u / C::PIECES % 2) * HALF + pi * (C::PER * 1024) + lane * 16;
             const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
             for (int w = 0; w < C::PER; w++) {
@@ -729,42 +736,46 @@ __global__ __launch_bounds__(64 * kv_tile_waves(NB, F32), kv_tile_fill(NB, F32))
                 *(kv_h8 *)(o + w * 1024) = h;
             }
         }
-        if (st < 8 * NB) *(uint4 *)(buf + 2 * HALF + st * 16) = rawd;
+        if (cg < CPT && lane < S2) *(uint4 *)(buf + cg * BUF + 2 * HALF + lane * 16) = rawd;
     };
 
     // every stream makes `turns` turns, the last maybe without a chunk
-    const int g0 = k.k_begin >> 5, g_end = (k.k_end + 31) >> 5;
-    const int turns = k.k_begin < k.k_end ? (g_end - g0 + KS - 1) / KS : 0;
-    int g = g0 + ks;
-    bool have = true, have_n = true;
-    if (turns > 0 && g < g_end) fetch(places.at(g, have));
+    constexpr int STEP = KS * CPT;
+    const int g0 = k.k_begin >> 5;
+    const int turns = k.k_begin < k.k_end ? (g_end - g0 + STEP - 1) / STEP : 0;
+    int g = g0 + ks * CPT;
+    bool have[CPT] = {}, have_n[CPT] = {};
+    if (turns > 0 && g < g_end) fetch(g, have);
     Cols cols;
     cols.start(a, k, k.c0 + cg * (16 * NT), lane);
     // this wave's own columns see no key from here on
     const int i_last = (min(cols.c0 + 16 * NT, k.ncols) - 1) / k.G;
     const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.len - k.nq + i_last + 1 : k.len);
-    uint8_t *const mine = smem + ks * BUF;  // buffer t of the stream at t · KS · BUF
+    uint8_t *const mine = smem + ks * (CPT * BUF);  // buffer t of the stream at t · STEP · BUF
     if (turns > 0) {
         if (g < g_end) convert(mine);
-        if (g + KS < g_end) fetch(places.at(g + KS, have_n));
+        if (g + STEP < g_end) fetch(g + STEP, have_n);
         __syncthreads();
-        for (int t = 0; t < turns; t++, g += KS) {
-            const kv_lds kb = (kv_lds)(mine + (t & 1) * (KS * BUF)), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
-            bool have_2 = have_n;
-            if (g + KS < g_end) {
-                convert(mine + (~t & 1) * (KS * BUF));
-                if (g + 2 * KS < g_end) fetch(places.at(g + 2 * KS, have_2));
+        for (int t = 0; t < turns; t++, g += STEP) {
+            bool have_2[CPT] = {};
+            if (g + STEP < g_end) {
+                convert(mine + (~t & 1) * (STEP * BUF));
+                if (g + 2 * STEP < g_end) fetch(g + 2 * STEP, have_2);
             }
-            if (32 * g < see_any)
+#pragma unroll 1
+            for (int c = 0; c < CPT; c++) {
+                if (32 * (g + c) >= see_any) break;
+                const kv_lds kb = (kv_lds)(mine + (t & 1) * (STEP * BUF) + c * BUF), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
                 cols.chunk(
-                    a, k.len, g, have, lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
+                    a, k, g + c, CPT > 1 && c ? have[CPT - 1] : have[0], lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
                     [&](int b) { return lds16(kd + b * 64 + ka * 16); },
                     [&](int i) { return __builtin_bit_cast(kv_h8, lds16(vb + i * 1024 + lane * 16)); },
                     [&](int b) { return lds16(vd + b * 64 + ka * 16); },
                     [&](int i) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + ((lane + 64 * i) % (NB * 16)) * 4); });
+            }
             __syncthreads();
-            have = have_n;
-            have_n = have_2;
+#pragma unroll
+            for (int c = 0; c < CPT; c++) have[c] = have_n[c], have_n[c] = have_2[c];
         }
     }
     cols.join_lanes();

@@ -17,8 +17,8 @@
 // stays below fp16's largest and well above its smallest, a column's exponents
 // are measured from a reference: its largest score so far plus the exponent of
 // the largest scale of V among the keys it has seen; both are taken again, and
-// the accumulators scaled, when a score exceeds its by 8 or a scale exceeds its
-// own (P·d ≤ 2^15 in between).
+// the accumulators scaled, when a score exceeds its by 6 or a scale is over
+// twice to four times the largest (P·d is at most 2^7 then, 2^15 in between).
 #pragma once
 
 #include "k_kv.h"
@@ -132,6 +132,9 @@ __device__ __forceinline__ uint32_t max_u16(uint32_t a, uint32_t b) {
     typedef uint16_t u2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, a), __builtin_bit_cast(u2, b)));
 }
+
+// 2^e as fp16 bits, e ≥ −24 (past fp16: larger than any).
+__device__ __forceinline__ uint32_t half_of(int e) { return e >= -14 ? (uint32_t)(e + 15) << 10 : 1u << (e + 24); }
 
 // s_waitcnt's field for at most n vector-memory operations under way.
 constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
@@ -416,22 +419,23 @@ struct KvColumns {
                 dm = max(dm & 0xffffu, dm >> 16);
                 dm = max(dm, (uint32_t)__shfl_xor((int)dm, 16, 64));
                 dm = max(dm, (uint32_t)__shfl_xor((int)dm, 32, 64));
-                // 2^e ≥ every scale: one above the exponent, or of a subnormal its bit length − 24
-                const int e = dm >= 0x400u ? (int)(dm >> 10) - 14 : 8 - (dm ? __builtin_clz(dm) : 32);
-                // the reference is the largest score + e − 7 (of a column that
+                // 2^e ≥ four times every scale (so that it is seldom outgrown): three
+                // above the exponent, or of a subnormal its bit length − 22
+                const int e = dm >= 0x400u ? (int)(dm >> 10) - 12 : 10 - (dm ? __builtin_clz(dm) : 32);
+                // the reference is the largest score + e − 9 (of a column that
                 // outgrew its own: what others see changes nothing of it)
-                const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (8.f - room[n]), up = max_over_keys(mx[n]);
-                const float top = fmaxf(best, up);
-                const bool mine = up > ref[n] + room[n] || (float)(15 - e) < room[n];
-                room[n] = fminf(room[n], (float)(15 - e));
-                const float ref_n = !mine ? ref[n] : (top <= KV_NONE ? KV_NONE : top + (8.f - room[n]));
-                const float alpha = ref_n == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - ref_n);
-                ref[n] = ref_n;
-                sum[n] *= alpha;
+                const float best = ref[n] == KV_NONE ? KV_NONE : ref[n] - (6.f - room[n]), up = max_over_keys(mx[n]);
+                if (up > ref[n] + room[n] || dm > half_of(15 - (int)room[n])) {
+                    const float top = fmaxf(best, up);
+                    room[n] = fminf(room[n], (float)(15 - e));
+                    const float ref_n = top <= KV_NONE ? KV_NONE : top + (6.f - room[n]);
+                    const float alpha = ref_n == ref[n] ? 1.f : __builtin_amdgcn_exp2f(ref[n] - ref_n);
+                    ref[n] = ref_n;
+                    sum[n] *= alpha;
 #pragma unroll
-                for (int w = 0; w < W; w++) acc[n][w] *= alpha;
-                const int ed = 15 - (int)room[n];
-                if (ref_n != KV_NONE) low = min(low, ed >= -14 ? (uint32_t)(ed + 15) << 10 : 1u << (ed + 24));
+                    for (int w = 0; w < W; w++) acc[n][w] *= alpha;
+                }
+                if (ref[n] != KV_NONE) low = min(low, half_of(15 - (int)room[n]));
             }
 #pragma unroll
             for (int x = 1; x < 16; x *= 2) low = min(low, (uint32_t)__shfl_xor((int)low, x, 64));

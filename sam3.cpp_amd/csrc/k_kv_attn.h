@@ -209,7 +209,7 @@ struct KvPlaces {
 };
 
 // NT · 16 columns of one wave: queries, running sums and output.
-template <int NB, bool F32, int NT, bool FENCE>
+template <int NB, bool F32, int NT, bool AHEAD>
 struct KvColumns {
     static constexpr int D = 32 * NB, W = 2 * NB;  // W: 16-channel tiles of V
     static constexpr int PARTS = F32 ? 2 : 1;      // fp16 operands of an fp32 value
@@ -328,7 +328,7 @@ struct KvColumns {
                     t[n][j] = __builtin_fmaf((float)kd[j], m[n][j >> 2][j & 3], b == 0 ? 0.f : t[n][j]);
                     __asm__ volatile("" : "+v"(t[n][j]));  // (here, not behind the next branch with every block's sums held)
                 }
-            if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
         uint32_t vds[VD];
 #pragma unroll
@@ -442,7 +442,10 @@ struct KvColumns {
             bound = __builtin_amdgcn_readfirstlane(low);
         }
 
-        // ---- probabilities, in units of the reference
+        // ---- probabilities, in units of the reference (AHEAD: V's first words on their way)
+        kv_h8 vw[2];
+        kv_u4 d;
+        if constexpr (AHEAD) vw[0] = vword(0), vw[1] = vword(1), d = vscale(0);
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
@@ -451,12 +454,14 @@ struct KvColumns {
                 sum[n] += t[n][j];
             }
 
-        // ---- Oᵀ += Vᵀ·(P·d)ᵀ, block by block of V's channels
+        // ---- Oᵀ += Vᵀ·(P·d)ᵀ, block by block of V's channels (AHEAD: the next block's words before this one's products)
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const kv_h8 vw[2] = {vword(2 * b), vword(2 * b + 1)};
+            if constexpr (!AHEAD) vw[0] = vword(2 * b), vw[1] = vword(2 * b + 1), d = vscale(b);
+            kv_h8 vn[2];
+            kv_u4 dn;
+            if (AHEAD && b + 1 < NB) vn[0] = vword(2 * b + 2), vn[1] = vword(2 * b + 3), dn = vscale(b + 1);
             kv_u4 p[NT][PARTS];
-            kv_u4 d = vscale(b);
             if (special) {
                 uint32_t h = all;
                 __asm__ volatile("" : "+v"(h));  // (nothing of this ahead of the branch)
@@ -498,7 +503,8 @@ struct KvColumns {
 #pragma unroll
                     for (int x = 0; x < PARTS; x++)
                         acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw[w & 1], __builtin_bit_cast(kv_h8, p[n][x]), acc[n][w], 0, 0, 0);
-            if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
+            if (AHEAD && b + 1 < NB) vw[0] = vn[0], vw[1] = vn[1], d = dn;
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
@@ -572,12 +578,12 @@ struct KvColumns {
 constexpr int KV_STAGES = 2, KV_WAVES = 4;
 // Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
 // through an accumulation register; more where the registers suffice.
-constexpr int kv_waves(int NB, int NT) { return NT > 1 || NB == 8 ? 2 : (NB <= 2 ? 4 : 3); }
+constexpr int kv_waves(int Q, int NB, int NT) { return NT > 1 || NB == 8 || Q * NB == 32 ? 2 : (NB <= 2 ? 4 : 3); }
 
 template <int Q, int NB, bool F32, int NT>
-__global__ __launch_bounds__(64 * KV_WAVES, kv_waves(NB, NT)) void k_kv_attn(KvAttnArgs a) {
+__global__ __launch_bounds__(64 * KV_WAVES, kv_waves(Q, NB, NT)) void k_kv_attn(KvAttnArgs a) {
     using C = KvChunk<Q, NB>;
-    using Cols = KvColumns<NB, F32, NT, true>;
+    using Cols = KvColumns<NB, F32, NT, false>;
     constexpr int W = Cols::W, WAVES = KV_WAVES;
     constexpr int LD = (C::BYTES + 1023) / 1024;  // 1 KB loads of a chunk
     // at the end the accumulators of two waves
@@ -665,148 +671,116 @@ __global__ __launch_bounds__(64 * KV_WAVES, kv_waves(NB, NT)) void k_kv_attn(KvA
     cols.store(a, k, lane);
 }
 
-// ---- many columns: bound by vector instructions ------------------------------
-// Eight waves: KS streams of them take every KS-th chunk, and the waves of a
-// stream hold columns of their own against the same chunks, whose words are
-// converted to fp16 once for all of them: each converts some while the chunk
-// before is worked on, into one of two buffers of whole MFMA operands (16 bytes
-// a lane and word, in the order of lanes, so neither side has bank conflicts).
-// One barrier a chunk.  Two streams halve the longest work-group (a causal
-// prompt's last columns see every key) and are joined in LDS; at head dim 256,
-// where that memory holds one stream's buffers, all eight share one.
-constexpr int kv_tile_waves(int NB, bool F32) { return NB == 8 && !F32 ? 12 : 8; }
-constexpr int kv_tile_nt(int NB, bool F32) { return F32 ? (NB <= 2 ? 2 : 1) : (NB == 8 ? 1 : 2); }
-constexpr int kv_tile_fill(int NB, bool F32) { return F32 ? 2 : (NB <= 2 ? 4 : (NB == 8 ? 3 : 2)); }
-constexpr int kv_tile_streams(int NB) { return NB == 8 ? 1 : 2; }
-constexpr int kv_tile_chunks(int NB) { return NB <= 2 ? 2 : 1; }
-constexpr int kv_tile_cols(int NB, bool F32) { return 16 * kv_tile_nt(NB, F32) * kv_tile_waves(NB, F32) / kv_tile_streams(NB); }
+// ---- many columns at head dim 256: bound by vector instructions and LDS -------
+// There a wave's registers hold no second column tile to share a chunk's
+// conversion with, and the first kernel's rings leave a CU one or two
+// work-groups.  Here the waves hold 16 columns each against the same chunks,
+// whose words are converted to fp16 once for all of them: each converts some
+// while the chunk before is worked on, into one of two buffers of whole MFMA
+// operands (16 bytes a lane and word, in the order of lanes, so neither side
+// has bank conflicts).  One barrier a chunk.  fp16 takes 12 waves in 168
+// registers, fp32 8 in 256.
+constexpr int KV_TILE_NB = 8;
+constexpr int kv_tile_waves(bool F32) { return F32 ? 8 : 12; }
+constexpr int kv_tile_cols(bool F32) { return 16 * kv_tile_waves(F32); }
 
-template <int Q, int NB, bool F32>
-__global__ __launch_bounds__(64 * kv_tile_waves(NB, F32), kv_tile_fill(NB, F32)) void k_kv_attn_tile(KvAttnArgs a) {
+template <int Q, bool F32>
+__global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) void k_kv_attn_tile(KvAttnArgs a) {
+    constexpr int NB = KV_TILE_NB, WAVES = kv_tile_waves(F32);
     using C = KvChunk<Q, NB>;
-    constexpr int NT = kv_tile_nt(NB, F32), KS = kv_tile_streams(NB), CG = kv_tile_waves(NB, F32) / KS, CPT = kv_tile_chunks(NB);
-    using Cols = KvColumns<NB, F32, NT, (NB > 4 || (!F32 && NB <= 2))>;
+    using Cols = KvColumns<NB, F32, 1, true>;
     constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
-    constexpr int W = Cols::W, BUFS = 2 * KS * CPT * BUF, JOIN = KS > 1 ? CG * NT * (W * 1024 + 512) : 0;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[BUFS > JOIN ? BUFS : JOIN];
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUF];
 
     const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ks = wave / CG, cg = wave % CG;  // stream, column group
     int s;
-    const KvTask k = kv_task<kv_tile_cols(NB, F32)>(a, s);
+    const KvTask k = kv_task<kv_tile_cols(F32)>(a, s);
     if (!k.some) return;
     const KvPlaces places(a, s, k.kvh, C::BYTES);
 
-    // pieces of K and V this wave converts; wave c of a stream takes chunk c's scales
-    constexpr int P2 = 2 * C::PIECES, PW = (CPT * P2 + CG - 1) / CG, S2 = 8 * NB;
-    static_assert(S2 <= 64 && CPT <= CG && CPT <= 2, "a wave for the scales of each chunk");
+    // pieces of K and V this wave converts; the scales are the last wave's (of fewer pieces)
+    constexpr int P2 = 2 * C::PIECES, PW = (P2 + WAVES - 1) / WAVES;
+    static_assert(8 * NB == 64 && C::WORDS % C::PER == 0, "16 bytes of scales a lane, whole pieces");
     uint4 raw[PW], rawd;
-    const int g_end = (k.k_end + 31) >> 5;
-    // chunks g .. g + CPT, as far as there are any; `have` their pages
-    auto fetch = [&](int g, bool *have) {
-        const uint8_t *p[CPT];
-#pragma unroll
-        for (int c = 0; c < CPT; c++) p[c] = places.at(CPT > 1 ? min(g + c, g_end - 1) : g, have[c]);
+    auto fetch = [&](const uint8_t *p) {
 #pragma unroll
         for (int i = 0; i < PW; i++) {
-            const int u = cg + i * CG, pi = u % C::PIECES;
-            if (u >= CPT * P2) continue;
-            const uint8_t *q = p[CPT > 1 && u >= P2 ? 1 : 0] + (u / C::PIECES % 2) * C::HALF + pi * 1024 + lane * (C::width(pi) * Q);
-            if (C::width(pi) == C::PER) {
-                raw[i] = gload16(q);
-            } else {
-                const uint2 x = gload8(q);
-                raw[i] = make_uint4(x.x, x.y, 0, 0);
-            }
+            const int u = wave + i * WAVES;
+            if (u < P2) raw[i] = gload16(p + (u / C::PIECES) * C::HALF + u % C::PIECES * 1024 + lane * 16);
         }
-        if (cg < CPT && lane < S2)
-            rawd = gload16(p[CPT > 1 && cg ? 1 : 0] + C::CODES + (lane < 4 * NB ? lane * 16 : C::HALF + (lane - 4 * NB) * 16));
+        if (wave == WAVES - 1) rawd = gload16(p + C::CODES + (lane < 32 ? lane * 16 : C::HALF + (lane - 32) * 16));
     };
     const KvMagic M;
     auto convert = [&](uint8_t *buf) {
 #pragma unroll
         for (int i = 0; i < PW; i++) {
-            const int u = cg + i * CG, pi = u % C::PIECES;
-            if (u >= CPT * P2) continue;
-            uint8_t *o = buf + (CPT > 1 && u >= P2 ? BUF : 0) + (u / C::PIECES % 2) * HALF + pi * (C::PER * 1024) + lane * 16;
+            const int u = wave + i * WAVES;
+            if (u >= P2) continue;
+            uint8_t *o = buf + u * (C::PER * 1024) + lane * 16;
             const uint32_t x[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
             for (int w = 0; w < C::PER; w++) {
-                if (w >= C::width(pi)) continue;
                 kv_h8 h;
                 if constexpr (Q == 4) h = word_h8_q4(x[w], M);
                 else h = word_h8_q8(x[2 * w], x[2 * w + 1]);
                 *(kv_h8 *)(o + w * 1024) = h;
             }
         }
-        if (cg < CPT && lane < S2) *(uint4 *)(buf + cg * BUF + 2 * HALF + lane * 16) = rawd;
+        if (wave == WAVES - 1) *(uint4 *)(buf + 2 * HALF + lane * 16) = rawd;
     };
 
-    // every stream makes `turns` turns, the last maybe without a chunk
-    constexpr int STEP = KS * CPT;
-    const int g0 = k.k_begin >> 5;
-    const int turns = k.k_begin < k.k_end ? (g_end - g0 + STEP - 1) / STEP : 0;
-    int g = g0 + ks * CPT;
-    bool have[CPT] = {}, have_n[CPT] = {};
-    if (turns > 0 && g < g_end) fetch(g, have);
+    const int g_end = (k.k_end + 31) >> 5;
+    int g = k.k_begin >> 5;
+    const int turns = k.k_begin < k.k_end ? g_end - g : 0;
+    bool have = true, have_n = true;
+    if (turns > 0) fetch(places.at(g, have));
     Cols cols;
-    cols.start(a, k, k.c0 + cg * (16 * NT), lane);
+    cols.start(a, k, k.c0 + wave * 16, lane);
     // this wave's own columns see no key from here on
-    const int i_last = (min(cols.c0 + 16 * NT, k.ncols) - 1) / k.G;
+    const int i_last = (min(cols.c0 + 16, k.ncols) - 1) / k.G;
     const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.len - k.nq + i_last + 1 : k.len);
-    uint8_t *const mine = smem + ks * (CPT * BUF);  // buffer t of the stream at t · STEP · BUF
     if (turns > 0) {
-        if (g < g_end) convert(mine);
-        if (g + STEP < g_end) fetch(g + STEP, have_n);
+        convert(smem);
+        if (g + 1 < g_end) fetch(places.at(g + 1, have_n));
         __syncthreads();
-        for (int t = 0; t < turns; t++, g += STEP) {
-            bool have_2[CPT] = {};
-            if (g + STEP < g_end) {
-                convert(mine + (~t & 1) * (STEP * BUF));
-                if (g + 2 * STEP < g_end) fetch(g + 2 * STEP, have_2);
+        for (int t = 0; t < turns; t++, g++) {
+            const kv_lds kb = (kv_lds)(smem + (t & 1) * BUF), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
+            bool have_2 = have_n;
+            if (g + 1 < g_end) {
+                convert(smem + (~t & 1) * BUF);
+                if (g + 2 < g_end) fetch(places.at(g + 2, have_2));
             }
-#pragma unroll 1
-            for (int c = 0; c < CPT; c++) {
-                if (32 * (g + c) >= see_any) break;
-                const kv_lds kb = (kv_lds)(mine + (t & 1) * (STEP * BUF) + c * BUF), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
+            if (32 * g < see_any)
                 cols.chunk(
-                    a, k, g + c, CPT > 1 && c ? have[CPT - 1] : have[0], lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
+                    a, k, g, have, lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
                     [&](int b) { return lds16(kd + b * 64 + ka * 16); },
                     [&](int i) { return __builtin_bit_cast(kv_h8, lds16(vb + i * 1024 + lane * 16)); },
                     [&](int b) { return lds16(vd + b * 64 + ka * 16); },
-                    [&](int i) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + ((lane + 64 * i) % (NB * 16)) * 4); });
-            }
+                    [&](int i) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + (lane + 64 * i) * 4); });
             __syncthreads();
-#pragma unroll
-            for (int c = 0; c < CPT; c++) have[c] = have_n[c], have_n[c] = have_2[c];
+            have = have_n;
+            have_n = have_2;
         }
     }
     cols.join_lanes();
-    if constexpr (KS > 1) {
-        // the second stream's sums into the first's (the last barrier left the buffers free)
-        uint8_t *const at = smem + cg * (NT * (W * 1024 + 512)) + lane * 16;
-        if (ks == 1) cols.give(at, lane);
-        __syncthreads();
-        if (ks == 1) return;
-        cols.take(at, lane);
-    }
     if (cols.c0 < k.ncols) cols.store(a, k, lane);
 }
 
 // Column tiles a wave of the first kernel holds where there are more than 16 columns.
-template <int NB, bool F32>
-constexpr int kv_most_tiles() { return NB == 8 ? 1 : 2; }
+constexpr int kv_most_tiles(int NB) { return NB == 8 ? 1 : 2; }
 
 template <int Q>
 hipError_t launch_kv_attn(const KvAttnArgs &a, bool f32, hipStream_t st) {
     const int64_t grid = ((int64_t)a.n_seq * a.c.heads * a.nsplit * a.ctiles + 7) / 8 * 8;
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     auto go = [&](auto nb, auto f) {
-        constexpr int NB = nb(), MOST = kv_most_tiles<NB, f()>();
+        constexpr int NB = nb(), MOST = kv_most_tiles(NB);
         const dim3 g((unsigned)grid);
-        if (a.tile) hipLaunchKernelGGL((k_kv_attn_tile<Q, NB, f()>), g, dim3(64 * kv_tile_waves(NB, f())), 0, st, a);
-        else if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), g, dim3(64 * KV_WAVES), 0, st, a);
+        if (a.tile) {
+            if constexpr (NB == KV_TILE_NB) hipLaunchKernelGGL((k_kv_attn_tile<Q, f()>), g, dim3(64 * kv_tile_waves(f())), 0, st, a);
+            else return hipErrorInvalidValue;
+        } else if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), g, dim3(64 * KV_WAVES), 0, st, a);
         else if (a.nt == MOST) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), MOST>), g, dim3(64 * KV_WAVES), 0, st, a);
         else return hipErrorInvalidValue;
         return hipGetLastError();

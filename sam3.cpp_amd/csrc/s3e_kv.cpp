@@ -108,6 +108,7 @@ constexpr int64_t KV_MIN_KEYS = 256;
 // alone, so that a captured call is the same for any lengths.
 void plan(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, bool f32, KvAttnArgs &a) {
     a.n_seq = (int)b->n_seq;
+    a.c.type = c->type;
     kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * (nh / c->n_heads));
     const int64_t wgs = b->n_seq * c->n_heads * a.ctiles;
     int64_t ns = a.tile ? a.goal / wgs : (a.goal + wgs - 1) / wgs;

@@ -676,9 +676,9 @@ __global__ __launch_bounds__(64 * KV_WAVES, kv_waves(Q, NB, NT)) void k_kv_attn(
 // conversion with, and the first kernel's rings leave a CU one or two
 // work-groups.  Here the waves hold 16 columns each against the same chunks,
 // whose words are converted to fp16 once for all of them: each converts some
-// while the chunk before is worked on, into one of two buffers of whole MFMA
+// while chunks before are worked on, into one of four buffers of whole MFMA
 // operands (16 bytes a lane and word, in the order of lanes, so neither side
-// has bank conflicts).  One barrier a chunk.  fp16 takes 12 waves in 168
+// has bank conflicts).  One barrier every two chunks.  fp16 takes 12 waves in 168
 // registers, fp32 8 in 256.
 constexpr int KV_TILE_NB = 8;
 constexpr int kv_tile_waves(bool F32) { return F32 ? 8 : 12; }
@@ -690,7 +690,7 @@ __global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) vo
     using C = KvChunk<Q, NB>;
     using Cols = KvColumns<NB, F32, 1, true>;
     constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * BUF];
+    __shared__ __attribute__((aligned(16))) uint8_t smem[4 * BUF];
 
     const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -731,36 +731,40 @@ __global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) vo
     };
 
     const int g_end = (k.k_end + 31) >> 5;
-    int g = k.k_begin >> 5;
-    const int turns = k.k_begin < k.k_end ? g_end - g : 0;
-    bool have = true, have_n = true;
-    if (turns > 0) fetch(places.at(g, have));
+    const int g0 = k.k_begin >> 5, n = k.k_begin < k.k_end ? g_end - g0 : 0;
+    // the pages of chunks i, i + 1, i + 2
+    bool have = true, have_1 = true, have_2 = true;
+    if (n > 0) fetch(places.at(g0, have));
     Cols cols;
     cols.start(a, k, k.c0 + wave * 16, lane);
     // this wave's own columns see no key from here on
     const int i_last = (min(cols.c0 + 16, k.ncols) - 1) / k.G;
     const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.len - k.nq + i_last + 1 : k.len);
-    if (turns > 0) {
+    if (n > 0) {
         convert(smem);
-        if (g + 1 < g_end) fetch(places.at(g + 1, have_n));
+        if (n > 1) {
+            fetch(places.at(g0 + 1, have_1));
+            convert(smem + BUF);
+        }
+        if (n > 2) fetch(places.at(g0 + 2, have_2));
         __syncthreads();
-        for (int t = 0; t < turns; t++, g++) {
-            const kv_lds kb = (kv_lds)(smem + (t & 1) * BUF), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
-            bool have_2 = have_n;
-            if (g + 1 < g_end) {
-                convert(smem + (~t & 1) * BUF);
-                if (g + 2 < g_end) fetch(places.at(g + 2, have_2));
+        for (int i = 0; i < n; i++) {
+            const kv_lds kb = (kv_lds)(smem + (i & 3) * BUF), vb = kb + HALF, kd = kb + 2 * HALF, vd = kd + C::SCALES;
+            bool have_3 = true;
+            if (i + 2 < n) {
+                convert(smem + (i + 2 & 3) * BUF);
+                if (i + 3 < n) fetch(places.at(g0 + i + 3, have_3));
             }
-            if (32 * g < see_any)
+            if (32 * (g0 + i) < see_any)
                 cols.chunk(
-                    a, k, g, have, lane, [&](int i) { return __builtin_bit_cast(kv_h8, lds16(kb + i * 1024 + lane * 16)); },
+                    a, k, g0 + i, have, lane, [&](int w) { return __builtin_bit_cast(kv_h8, lds16(kb + w * 1024 + lane * 16)); },
                     [&](int b) { return lds16(kd + b * 64 + ka * 16); },
-                    [&](int i) { return __builtin_bit_cast(kv_h8, lds16(vb + i * 1024 + lane * 16)); },
+                    [&](int w) { return __builtin_bit_cast(kv_h8, lds16(vb + w * 1024 + lane * 16)); },
                     [&](int b) { return lds16(vd + b * 64 + ka * 16); },
-                    [&](int i) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + (lane + 64 * i) * 4); });
-            __syncthreads();
-            have = have_n;
-            have_n = have_2;
+                    [&](int w) { return *(__attribute__((address_space(3))) const uint32_t *)(vd + (lane + 64 * w) * 4); });
+            // chunk i + 2 takes the buffer of i − 2: apart by a barrier, as i + 2 and its conversion are
+            if (i & 1) __syncthreads();
+            have = have_1, have_1 = have_2, have_2 = have_3;
         }
     }
     cols.join_lanes();

@@ -169,9 +169,9 @@ constexpr int KV_ROWS = 64;  // rows of a work-group, four threads each
 // channel: where eight rows of the call fill one aligned run of eight slots
 // their codes meet in LDS and the words are stored whole, by the work-group
 // whose rows hold the run's first (it converts up to seven of the next one's
-// rows again); a row outside any run replaces its own code in each word, a
-// nibble by an atomic and and or, a byte by a byte store, so that runs, lone
-// rows and neighbouring work-groups never write each other's codes.
+// rows again); a row outside any run replaces its own code in each word by a
+// 64-bit atomic or a byte store, so that runs, lone rows and neighbouring
+// work-groups never write each other's codes.
 // Bound by HBM: the rows are read once and the words written once.
 template <int Q, int NB, typename T>
 __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
     // rows −7 .. 64 + 13 of the call's slots around this work-group's
     __shared__ int32_t sl[KV_ROWS + 21];
     __shared__ uint8_t codes_lds[(KV_ROWS + 7) * D];
-    __shared__ int starts[KV_ROWS / 8 + 1];
+    __shared__ int starts[KV_ROWS / 8 + 1], lones[KV_ROWS + 1];
     const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
     const int64_t r0 = (int64_t)blockIdx.x * KV_ROWS;
@@ -248,34 +248,17 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
         return;
     }
 
-    // V: own rows, then those of the next work-group that a run from here ends in
+    // V: own rows' codes, then those of the next work-group that a run from here ends in
     auto convert = [&](int r, bool own, const Raw8<T> *raw) {
         const int s = sl[r + 7];
-        const bool run = in_run(r);
         uint8_t *cv = chunk_of(a.c, s, head, C::BYTES) + C::HALF;
-        const int key = s & 31;
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             uint32_t c[8];
             uint16_t d;
             quant_block<Q>(raw[b], lane, c, d);
-            if (own && g == (b & 3)) *(uint16_t *)(cv + C::CODES + (b * 32 + key) * 2) = d;
-            if (run) {
-                *(uint2 *)(codes_lds + r * D + 32 * b + 8 * g) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int ch = 32 * b + 8 * g + j, k8 = key & 7;
-                    uint8_t *p = cv + C::word(ch >> 4, 16 * (key >> 3) + (ch & 15));
-                    if constexpr (Q == 4) {
-                        const int sft = 4 * ((k8 >> 1) + 4 * (k8 & 1));
-                        atomicAnd((uint32_t *)p, ~(15u << sft));
-                        atomicOr((uint32_t *)p, c[j] << sft);
-                    } else {
-                        p[k8] = (uint8_t)c[j];
-                    }
-                }
-            }
+            if (own && g == (b & 3)) *(uint16_t *)(cv + C::CODES + (b * 32 + (s & 31)) * 2) = d;
+            *(uint2 *)(codes_lds + r * D + 32 * b + 8 * g) = make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
         }
     };
     if (sl[(tid >> 2) + 7] >= 0) convert(tid >> 2, true, own_row);
@@ -289,12 +272,34 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
         }
     }
     if (tid < 64) {
-        const bool first = (sl[tid + 7] & 7) == 0 && in_run(tid);
-        const uint64_t m = __ballot(first);
-        if (first) starts[1 + __popcll(m & ((1ull << tid) - 1))] = tid;
-        if (tid == 0) starts[0] = __popcll(m);
+        const bool run = in_run(tid), first = run && (sl[tid + 7] & 7) == 0, lone = !run && sl[tid + 7] >= 0;
+        const uint64_t below = (1ull << tid) - 1, m = __ballot(first), o = __ballot(lone);
+        if (first) starts[1 + __popcll(m & below)] = tid;
+        if (lone) lones[1 + __popcll(o & below)] = tid;
+        if (tid == 0) starts[0] = __popcll(m), lones[0] = __popcll(o);
     }
     __syncthreads();
+    // lone rows: unit (row, piece, channel m of 16), the row's own code in each of
+    // the lane's words.  Others of the call may share a word: a nibble is
+    // exchanged by one xor with what it has to change (nobody else writes it, so
+    // what is read of it stands), a byte is stored
+    for (int u = tid; u < lones[0] * C::PIECES * 16; u += 256) {
+        const int m = u & 15, pi = (u >> 4) % C::PIECES, r = lones[1 + (u >> 4) / C::PIECES];
+        const int s = sl[r + 7], k8 = s & 7;
+        uint8_t *o = chunk_of(a.c, s, head, C::BYTES) + C::HALF + C::word(pi * C::PER, 16 * ((s & 31) >> 3) + m);
+        const uint8_t *c = codes_lds + r * D + 16 * pi * C::PER + m;
+        if constexpr (Q == 4) {
+            const int sft = 4 * ((k8 >> 1) + 4 * (k8 & 1));
+            const bool whole = C::width(pi) == C::PER;
+            const uint2 lo = *(const uint2 *)o, hi = whole ? *(const uint2 *)(o + 8) : make_uint2(0, 0);
+            auto change = [&](uint32_t old, int w) { return (old ^ (uint32_t)c[16 * w] << sft) & 15u << sft; };
+            atomicXor((unsigned long long *)o, change(lo.x, 0) | (unsigned long long)change(lo.y, 1) << 32);
+            if (whole) atomicXor((unsigned long long *)(o + 8), change(hi.x, 2) | (unsigned long long)change(hi.y, 3) << 32);
+        } else {
+#pragma unroll
+            for (int w = 0; w < C::PER; w++) o[8 * w + k8] = c[16 * w];
+        }
+    }
     // whole words: unit (run, piece, four channels 4q .. 4q + 4 of 16).  The bytes
     // of four channels come as one word a row; two rows' nibbles share its bytes,
     // and a 4 × 4 transpose of bytes turns four such words into a channel's each

@@ -508,3 +508,92 @@ def test_captured_decoding(ctx, io):
             gr.h.hipGraphExecDestroy(ex)
             gr.h.hipGraphDestroy(g)
         gr.h.hipStreamDestroy(other)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("kv", [20, 33, 65, 97, 700])
+def test_many_columns_of_256(ctx, t, io, kv):
+    # the kernel for many columns at head dim 256: odd and even numbers of chunks, one of them, several key ranges,
+    # a last work-group with few columns, rows that see nothing
+    Batch(ctx, t, io, 1, 2, 256, 32, [(150, kv)], seed=kv).check()
+    Batch(ctx, t, io, 1, 2, 256, 64, [(3, 5), (131, kv)], seed=kv, mask=True, causal=False).check()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_a_key_hidden_from_some_of_many_columns(ctx, t):
+    kv, nq, D = 100, 300, 256
+    x = Batch(ctx, t, s3e.TYPE_F16, 1, 1, D, 64, [(nq, kv)], seed=nq, mask=True, causal=False)
+    x.mask[:] = 0
+    x.mask[::2, 33] = -np.inf
+    x.md.upload(x.mask)
+    table = x.arrays[2].download(np.int32, (1, 2))
+    slots = np.array([table[0, j // 64] * 64 + j % 64 for j in range(kv)], np.int32)
+    v = x.v.copy()
+    v[33] = np.nan
+    ctx.kv_write(x.c, s3e.TYPE_F32, ctx.to_device(x.k), (D, D), ctx.to_device(v), (D, D), ctx.to_device(slots), kv)
+    got = x.run()
+    want, bound = x.want()
+    assert np.isnan(got[1::2]).all()
+    assert (np.abs(got[::2].astype(np.float64) - want[::2]) <= bound[::2]).all()
+
+
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("nq", [1, 20])
+def test_many_sequences(ctx, io, nq):
+    # 203 of them, some without queries, some without keys, in a number that no XCD's share divides
+    rng = np.random.default_rng(nq)
+    lens = [(int(rng.integers(0, nq + 1)), int(rng.integers(0, 80))) for _ in range(203)]
+    Batch(ctx, ref.Q4_0, io, 1, 3, 32, 32, lens, seed=5, max_q=nq).check()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+def test_writers_of_neighbouring_slots_at_once(ctx, t, io):
+    # two contexts write every other slot, so that each word of V holds codes of both, and runs beside lone rows
+    rng = np.random.default_rng(31)
+    heads, D, page, n_pages = 2, 96, 64, 5
+    n = n_pages * page // 2
+    other = s3e.Context()
+    c, mem = make_cache(ctx, t, heads, D, page, n_pages, rng)
+    nb = (heads * D, D)
+    calls = []
+    for cx, slots in ((ctx, np.arange(0, 2 * n, 2)), (other, np.arange(1, 2 * n, 2))):
+        slots = slots.astype(np.int32)
+        if cx is ctx:
+            slots = rng.permutation(slots)
+        k, v = rows(rng, n, heads, D, io), rows(rng, n, heads, D, io)
+        ref.write(mem, t, D, page, heads, slots, k.astype(np.float32), v.astype(np.float32))
+        calls.append((cx, cx.to_device(k), cx.to_device(v), cx.to_device(slots)))
+    for cx, _, _, _ in calls:
+        cx.sync()
+    for _ in range(3):
+        for cx, kd, vd, sd in calls:
+            cx.kv_write(c, io, kd, nb, vd, nb, sd, n)
+    for cx, _, _, _ in calls:
+        cx.sync()
+    assert np.array_equal(c._data.download(np.uint8, mem.shape), mem)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("lone", [False, True])
+def test_a_slot_given_twice_harms_no_other(ctx, t, lone):
+    rng = np.random.default_rng(8)
+    heads, D, page = 2, 64, 32
+    c, mem = make_cache(ctx, t, heads, D, page, 3, rng)
+    # slot 5 twice: among scattered rows, or in a run of eight and again behind it
+    slots = np.array([5, 40, 70, 5, 2, 3] if lone else list(range(8, 16)) + list(range(0, 8)) + [5], np.int32)
+    n = len(slots)
+    k, v = rows(rng, n, heads, D, s3e.TYPE_F32), rows(rng, n, heads, D, s3e.TYPE_F32)
+    nb = (heads * D, D)
+    ctx.kv_write(c, s3e.TYPE_F32, ctx.to_device(k), nb, ctx.to_device(v), nb, ctx.to_device(slots), n)
+    ctx.sync()
+    got = c._data.download(np.uint8, mem.shape)
+    ref.write(mem, t, D, page, heads, slots, k, v)
+    # whatever slot 5 holds, write it again on both sides
+    again = np.array([5], np.int32)
+    c._data.upload(got)
+    ctx.kv_write(c, s3e.TYPE_F32, ctx.to_device(k[:1]), nb, ctx.to_device(v[:1]), nb, ctx.to_device(again), 1)
+    ctx.sync()
+    ref.write(mem, t, D, page, heads, again, k[:1], v[:1])
+    assert np.array_equal(c._data.download(np.uint8, mem.shape), mem)

@@ -167,8 +167,11 @@ __device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
         unit = at / a.ctiles;
         ct = a.ctiles - 1 - at % a.ctiles;
     }
-    const int sh = unit / a.nsplit;
-    t.split = unit % a.nsplit;
+    // (every sequence's first range, then the second of those that have one: the
+    // short ones last; sequence by sequence a batch of 64 took 53 µs, so 51)
+    const int shs = a.n_seq * a.c.heads;
+    t.split = unit / shs;
+    const int sh = unit - t.split * shs;
     s = sh / a.c.heads;
     t.kvh = sh - s * a.c.heads;
     t.G = a.nh / a.c.heads;
@@ -577,7 +580,7 @@ struct KvColumns {
 // under way without holding registers, so that two to four work-groups share a
 // CU and no wave waits for another before the end.
 // One token of 64 sequences of up to 4096 keys (8 heads of 128, 32 query heads,
-// Q4_0, 174 MB) takes 53 µs with the joining pass, 3.3 TB/s; one of 131 072 keys
+// Q4_0, 174 MB) takes 51 µs with the joining pass, 3.4 TB/s; one of 131 072 keys
 // (151 MB) 41 µs, 3.7 TB/s.  Vector instructions, half of them the conversion of
 // codes to fp16, are busy 55 % of the cycles there and wait on one another, on
 // the longest range and on memory for the rest.  4 × 2048 causal queries over up

@@ -336,7 +336,7 @@ int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t 
  * Q(row, h, d) = q[row·q_nb[0] + h·q_nb[1] + d]; o is [n_tokens][nh][D]
  * (16-byte aligned), of the same `type`:
  *   S3E_TYPE_F16  q in fp16, probabilities times V's scales rounded to fp16
- *                 (fp32 scores, sums and accumulation);
+ *                 where max_kv is over 128 (fp32 scores, sums and accumulation);
  *   S3E_TYPE_F32  q and those products as fp16 pairs: fp32 attention to ~1e-6.
  * causal: row i of a sequence's nq sees keys 0 .. kv_len − nq + i; otherwise
  * all kv_len of them.  mask (NULL: none): fp16, mask[row·mask_ld + key] is

@@ -212,10 +212,13 @@ struct KvPlaces {
 };
 
 // NT · 16 columns of one wave: queries, running sums and output.
-template <int NB, bool F32, int NT, bool AHEAD>
+// PAIRS: P·d as fp16 pairs too (fp32 operands: always).
+template <int NB, bool F32, int NT, bool AHEAD, bool PAIRS>
 struct KvColumns {
     static constexpr int D = 32 * NB, W = 2 * NB;  // W: 16-channel tiles of V
     static constexpr int PARTS = F32 ? 2 : 1;      // fp16 operands of an fp32 value
+    static constexpr int PP = PAIRS ? 2 : 1;       // of a P·d
+    static_assert(PAIRS || !F32, "fp32 is pairs throughout");
     static constexpr int VD = (NB * 16 + 63) / 64;
 
     int c0, see_all;
@@ -464,7 +467,7 @@ struct KvColumns {
             kv_h8 vn[2];
             kv_u4 dn;
             if (AHEAD && b + 1 < NB) vn[0] = vword(2 * b + 2), vn[1] = vword(2 * b + 3), dn = vscale(b + 1);
-            kv_u4 p[NT][PARTS];
+            kv_u4 p[NT][PP];
             if (special) {
                 uint32_t h = all;
                 __asm__ volatile("" : "+v"(h));  // (nothing of this ahead of the branch)
@@ -473,7 +476,7 @@ struct KvColumns {
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                if constexpr (!F32) {
+                if constexpr (!PAIRS) {
                     p[n][0] = scaled_eight(t[n], d);
                 } else {
 #pragma unroll
@@ -484,7 +487,7 @@ struct KvColumns {
                         __asm__("" : "+v"(x), "+v"(y));
                         const kv_h2 hi = {(_Float16)x, (_Float16)y};
                         p[n][0][j] = __builtin_bit_cast(uint32_t, hi);
-                        p[n][PARTS - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
+                        p[n][PP - 1][j] = __builtin_bit_cast(uint32_t, kv_h2{(_Float16)(x - (float)hi[0]), (_Float16)(y - (float)hi[1])});
                     }
                 }
             }
@@ -494,7 +497,7 @@ struct KvColumns {
                     uint32_t h = hidden[n];
                     __asm__ volatile("" : "+v"(h));  // (nothing of this ahead of the branch)
 #pragma unroll
-                    for (int x = 0; x < PARTS; x++)
+                    for (int x = 0; x < PP; x++)
 #pragma unroll
                         for (int j = 0; j < 4; j++) p[n][x][j] &= keep_pair(h, j);
                 }
@@ -504,7 +507,7 @@ struct KvColumns {
 #pragma unroll
                 for (int n = 0; n < NT; n++)
 #pragma unroll
-                    for (int x = 0; x < PARTS; x++)
+                    for (int x = 0; x < PP; x++)
                         acc[n][w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vw[w & 1], __builtin_bit_cast(kv_h8, p[n][x]), acc[n][w], 0, 0, 0);
             if (AHEAD && b + 1 < NB) vw[0] = vn[0], vw[1] = vn[1], d = dn;
             __builtin_amdgcn_sched_barrier(0);
@@ -591,10 +594,10 @@ constexpr int KV_STAGES = 2, KV_WAVES = 4;
 // through an accumulation register; more where the registers suffice.
 constexpr int kv_waves(int Q, int NB, int NT) { return NT > 1 || NB == 8 || Q * NB == 32 ? 2 : (NB <= 2 ? 4 : 3); }
 
-template <int Q, int NB, bool F32, int NT>
+template <int Q, int NB, bool F32, int NT, bool PAIRS>
 __global__ __launch_bounds__(64 * KV_WAVES, kv_waves(Q, NB, NT)) void k_kv_attn(KvAttnArgs a) {
     using C = KvChunk<Q, NB>;
-    using Cols = KvColumns<NB, F32, NT, false>;
+    using Cols = KvColumns<NB, F32, NT, false, PAIRS>;
     constexpr int W = Cols::W, WAVES = KV_WAVES;
     constexpr int LD = (C::BYTES + 1023) / 1024;  // 1 KB loads of a chunk
     // at the end the accumulators of two waves
@@ -703,7 +706,7 @@ template <int Q, bool F32>
 __global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) void k_kv_attn_tile(KvAttnArgs a) {
     constexpr int NB = KV_TILE_NB, WAVES = kv_tile_waves(F32);
     using C = KvChunk<Q, NB>;
-    using Cols = KvColumns<NB, F32, 1, true>;
+    using Cols = KvColumns<NB, F32, 1, true, F32>;
     constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
     __shared__ __attribute__((aligned(16))) uint8_t smem[4 * BUF];
 
@@ -799,8 +802,17 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, bool f32, hipStream_t st) {
         if (a.tile) {
             if constexpr (NB == KV_TILE_NB) hipLaunchKernelGGL((k_kv_attn_tile<Q, f()>), g, dim3(64 * kv_tile_waves(f())), 0, st, a);
             else return hipErrorInvalidValue;
-        } else if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), g, dim3(64 * KV_WAVES), 0, st, a);
-        else if (a.nt == MOST) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), MOST>), g, dim3(64 * KV_WAVES), 0, st, a);
+        } else if (a.nt == 1 || a.nt == MOST) {
+            auto rings = [&](auto nt, auto pairs) {
+                hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), nt(), pairs()>), g, dim3(64 * KV_WAVES), 0, st, a);
+            };
+            auto by_pairs = [&](auto nt) {
+                if (f() || a.pairs) rings(nt, std::true_type{});
+                else if constexpr (!f()) rings(nt, std::false_type{});
+            };
+            if (a.nt == 1) by_pairs(std::integral_constant<int, 1>{});
+            else by_pairs(std::integral_constant<int, MOST>{});
+        }
         else return hipErrorInvalidValue;
         return hipGetLastError();
     };

@@ -597,3 +597,22 @@ def test_a_slot_given_twice_harms_no_other(ctx, t, lone):
     ctx.sync()
     ref.write(mem, t, D, page, heads, again, k[:1], v[:1])
     assert np.array_equal(c._data.download(np.uint8, mem.shape), mem)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("nq,kv", [(1, 2), (1, 128), (7, 40), (30, 128)])
+def test_few_keys_in_fp16_round_once(ctx, t, D, nq, kv):
+    # up to 128 keys: the products with V's scales are pairs as in fp32, and the output's rounding to fp16 (2^-11, and
+    # 2^-25 below its normal numbers) is all that is added to fp32's bound
+    x = Batch(ctx, t, s3e.TYPE_F16, 1, 2, D, 64, [(nq, kv), (nq, nq)], seed=D + kv, max_kv=max(kv, nq))
+    got = x.run().astype(np.float64)
+    at = 0
+    for i, (n, keys) in enumerate(x.lens):
+        parts = [p[at:at + keys] for y in (x.k, x.v) for p in ref.quantize(t, y)]
+        at += keys
+        see = np.arange(keys) <= (keys - n + np.arange(n)[:, None])
+        q = x.q[x.starts[i]:x.starts[i + 1], :2 * D].reshape(n, 2, D)
+        o, mag, A = ref.attention(t, *parts, q, x.scale, see)
+        bound = ref.attention_bound(True, o, mag, A, keys, D, ref.largest(t, *parts[2:]))
+        assert (np.abs(got[x.starts[i]:x.starts[i + 1]] - o) <= bound * (1 + 2.0 ** -11) + np.abs(o) * 2.0 ** -11 + 2.0 ** -25).all()

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
     constexpr int D = 32 * NB;
     // rows −7 .. 64 + 13 of the call's slots around this work-group's
     __shared__ int32_t sl[KV_ROWS + 21];
-    __shared__ uint8_t codes_lds[(KV_ROWS + 7) * D];
+    __shared__ __attribute__((aligned(16))) uint8_t codes_lds[(KV_ROWS + 7) * D];
     __shared__ int starts[KV_ROWS / 8 + 1], lones[KV_ROWS + 1];
     const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
     const bool is_v = blockIdx.z != 0;
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
     using C = KvChunk<Q, NB>;
     constexpr int D = 32 * NB;
     __shared__ int32_t sl[KV_ROWS];
-    __shared__ uint8_t codes_lds[KV_ROWS * D];
+    __shared__ __attribute__((aligned(16))) uint8_t codes_lds[KV_ROWS * D];
     __shared__ uint16_t scales_lds[KV_ROWS * NB];
     __shared__ uint64_t runs;
     const int tid = threadIdx.x, head = blockIdx.y;

@@ -139,6 +139,10 @@ __device__ __forceinline__ uint32_t half_of(int e) { return e >= -14 ? (uint32_t
 // s_waitcnt's field for at most n vector-memory operations under way.
 constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
+// Of the batch's arrays: read by scalar loads (a vector load would wait behind
+// every chunk under way).
+typedef __attribute__((address_space(4))) const int32_t c_i32;
+
 // What a work-group is to do: its sequence, key/value head, key range and
 // first column; `some` where there is anything.
 struct KvTask {
@@ -155,26 +159,41 @@ __device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
     // short ones fill the gaps
     KvTask t;
     t.some = false;
-    const int units = a.n_seq * a.c.heads * a.nsplit, total = units * a.ctiles, per = (total + 7) >> 3;
+    const int shs = (a.tiles ? 1 : a.n_seq) * a.c.heads, ctiles = a.tiles ? a.tiles : a.ctiles;
+    const int units = shs * a.nsplit, total = units * ctiles, per = (total + 7) >> 3;
     const int i = blockIdx.x >> 3, at = (blockIdx.x & 7) * per + i;
     if (i >= per || at >= total) return t;
     int unit, ct;
     if (units % 8 == 0) {
         const int u = units >> 3;
         unit = (i % u) * 8 + (blockIdx.x & 7);  // (dealt out: a long sequence's heads to every XCD)
-        ct = a.ctiles - 1 - i / u;
+        ct = ctiles - 1 - i / u;
     } else {
-        unit = at / a.ctiles;
-        ct = a.ctiles - 1 - at % a.ctiles;
+        unit = at / ctiles;
+        ct = ctiles - 1 - at % ctiles;
     }
     // (every sequence's first range, then the second of those that have one: the
     // short ones last; sequence by sequence a batch of 64 took 53 µs, so 51)
-    const int shs = a.n_seq * a.c.heads;
     t.split = unit / shs;
     const int sh = unit - t.split * shs;
     s = sh / a.c.heads;
     t.kvh = sh - s * a.c.heads;
-    t.G = a.nh / a.c.heads;
+    const int G = a.nh / a.c.heads;
+    if (a.tiles) {
+        // tiles of all sequences: s begins at q_start[s]·G / COLS + s, which leaves each
+        // at least as many as it has
+        const c_i32 *starts = (c_i32 *)a.q_start;
+        auto first = [&](int x) { return min(max(starts[x], 0), a.n_tokens) * G / COLS + x; };
+        int end = a.n_seq;
+        while (end - s > 1) {
+            const int mid = (s + end) >> 1;
+            if (first(mid) <= ct) s = mid;
+            else end = mid;
+        }
+        ct -= first(s);
+        if (ct < 0) return t;
+    }
+    t.G = G;
     t.q0 = min(max(a.q_start[s], 0), a.n_tokens);
     t.nq = min(max(a.q_start[s + 1], t.q0), a.n_tokens) - t.q0;
     t.ncols = min(t.nq, a.max_q) * t.G;
@@ -192,8 +211,6 @@ __device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
 
 // Where a sequence's chunks lie.
 struct KvPlaces {
-    // (read by scalar loads: a vector load would wait behind every chunk under way)
-    typedef __attribute__((address_space(4))) const int32_t c_i32;
     const c_i32 *pages;
     const uint8_t *base;     // of this head in page 0
     int64_t stride;          // bytes from page to page
@@ -794,7 +811,7 @@ constexpr int kv_most_tiles(int NB) { return NB == 8 ? 1 : 2; }
 
 template <int Q>
 hipError_t launch_kv_attn(const KvAttnArgs &a, bool f32, hipStream_t st) {
-    const int64_t grid = ((int64_t)a.n_seq * a.c.heads * a.nsplit * a.ctiles + 7) / 8 * 8;
+    const int64_t grid = ((int64_t)a.c.heads * a.nsplit * (a.tiles ? a.tiles : (int64_t)a.n_seq * a.ctiles) + 7) / 8 * 8;
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     auto go = [&](auto nb, auto f) {
         constexpr int NB = nb(), MOST = kv_most_tiles(NB);

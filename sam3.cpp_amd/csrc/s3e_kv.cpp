@@ -111,8 +111,9 @@ constexpr int64_t KV_MIN_KEYS = 256;
 void plan(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, bool f32, KvAttnArgs &a) {
     a.n_seq = (int)b->n_seq;
     a.c.type = c->type;
-    kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * (nh / c->n_heads), b->max_kv);
-    const int64_t wgs = b->n_seq * c->n_heads * a.ctiles;
+    const int64_t G = nh / c->n_heads;
+    kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * G, b->n_tokens * G, b->max_kv);
+    const int64_t wgs = c->n_heads * (a.tiles ? a.tiles : b->n_seq * a.ctiles);
     // (to the nearest: 64 sequences of up to 4096 keys, 16 heads of 64, Q8_0, whose
     // 1024 work-groups are two thirds of the goal, take 64 µs in one range, 70 in two)
     int64_t ns = (a.goal + (a.tile ? 0 : (wgs - 1) / 2)) / wgs;

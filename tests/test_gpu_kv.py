@@ -616,3 +616,16 @@ def test_few_keys_in_fp16_round_once(ctx, t, D, nq, kv):
         o, mag, A = ref.attention(t, *parts, q, x.scale, see)
         bound = ref.attention_bound(True, o, mag, A, keys, D, ref.largest(t, *parts[2:]))
         assert (np.abs(got[x.starts[i]:x.starts[i + 1]] - o) <= bound * (1 + 2.0 ** -11) + np.abs(o) * 2.0 ** -11 + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D", [32, 128, 256])
+@pytest.mark.parametrize("at", [0, 4, 9])
+def test_a_prompt_among_single_tokens(ctx, t, io, D, at):
+    # work-groups that look their sequence up: the prompt first, inside or last, sequences without rows or keys, several
+    # key ranges, more rows than the sequences have
+    tokens = [(1, 90), (1, 3), (0, 40), (1, 1000), (2, 2), (1, 0), (0, 0), (1, 31), (1, 257)]
+    lens = tokens[:at] + [(130, 200)] + tokens[at:]
+    for heads, nh, more in ((1, 3, {}), (8, 8, {"spare_rows": 5, "mask": True, "causal": False})):
+        Batch(ctx, t, io, heads, nh, D, 64, lens, seed=at + D, **more).check()

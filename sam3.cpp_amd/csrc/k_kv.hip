@@ -512,18 +512,30 @@ __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {
 // Bound by launch and two loads one behind the other where rows are few (32 rows
 // of 128 from 43 ranges 5.2 µs), by memory where they are many (4096 rows of 256
 // from 11 ranges, 47 MB: 12 µs).
-template <int D, bool F32, bool SPREAD>
+template <int D, bool F32, bool SPREAD, bool FIND>
 __global__ __launch_bounds__(256) void k_kv_combine(KvAttnArgs a) {
     constexpr int LANES = D / 4, GROUPS = 256 / LANES;
     __shared__ float4 acc_lds[SPREAD ? GROUPS : 1][LANES];
     __shared__ float sum_lds[GROUPS];
-    const int tid = threadIdx.x, s = blockIdx.y;
-    const int q0 = min(max(a.q_start[s], 0), a.n_tokens), q1 = min(max(a.q_start[s + 1], q0), a.n_tokens);
-    const int gr = tid / LANES, d4 = tid % LANES;
+    const int tid = threadIdx.x, gr = tid / LANES, d4 = tid % LANES;
     const int r = SPREAD ? blockIdx.x : blockIdx.x * GROUPS + gr;
-    const int i = r / a.nh, h = r - i * a.nh;
+    int i = r / a.nh, s = blockIdx.y;
+    const int h = r - i * a.nh;
     // (of a spread row all threads leave or none; GROUPS · LANES may be less than 256)
-    if (i >= min(q1 - q0, a.max_q) || (!SPREAD && gr >= GROUPS)) return;
+    if (!SPREAD && gr >= GROUPS) return;
+    if (FIND) {
+        // i is a row of all sequences': s the last that begins at or before it
+        if (i >= a.n_tokens) return;
+        int end = a.n_seq;
+        while (end - s > 1) {
+            const int mid = (s + end) >> 1;
+            if (a.q_start[mid] <= i) s = mid;
+            else end = mid;
+        }
+    }
+    const int q0 = min(max(a.q_start[s], 0), a.n_tokens), q1 = min(max(a.q_start[s + 1], q0), a.n_tokens);
+    if (FIND) i -= q0;
+    if (i < 0 || i >= min(q1 - q0, a.max_q)) return;
     const int64_t len = min((int64_t)max(a.kv_len[s], 0), a.max_kv);
     const int n = (int)min((len + a.chunk - 1) / a.chunk, (int64_t)a.nsplit);
     const int64_t row = (int64_t)(q0 + i) * a.nh + h, rows = (int64_t)a.n_tokens * a.nh;
@@ -619,11 +631,16 @@ hipError_t launch_kv_read(const KvReadArgs &a, bool f32, hipStream_t st) {
 hipError_t launch_kv_combine(const KvAttnArgs &a, bool f32, hipStream_t st) {
     auto go = [&](auto d, auto f) {
         constexpr int GROUPS = 256 / (d() / 4);
-        const int64_t rows = (int64_t)a.max_q * a.nh;
-        if (a.nsplit > 8)
-            hipLaunchKernelGGL((k_kv_combine<d(), f(), true>), dim3((unsigned)rows, a.n_seq), dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((k_kv_combine<d(), f(), false>), dim3((unsigned)((rows + GROUPS - 1) / GROUPS), a.n_seq), dim3(256), 0, st, a);
+        // rows of each sequence up to max_q, or, where that is over twice as many as
+        // there are, of all sequences, each of which is looked up
+        const bool find = a.n_seq > 1 && (int64_t)a.n_seq * a.max_q > 2 * (int64_t)a.n_tokens;
+        const int64_t rows = (int64_t)(find ? a.n_tokens : a.max_q) * a.nh;
+        auto run = [&](auto spread, auto look) {
+            const dim3 grid((unsigned)(spread() ? rows : (rows + GROUPS - 1) / GROUPS), find ? 1 : a.n_seq);
+            hipLaunchKernelGGL((k_kv_combine<d(), f(), spread(), look()>), grid, dim3(256), 0, st, a);
+        };
+        auto by_find = [&](auto spread) { find ? run(spread, std::true_type{}) : run(spread, std::false_type{}); };
+        a.nsplit > 8 ? by_find(std::true_type{}) : by_find(std::false_type{});
         return hipGetLastError();
     };
     auto by = [&](auto d) { return f32 ? go(d, std::true_type{}) : go(d, std::false_type{}); };

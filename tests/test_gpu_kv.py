@@ -629,3 +629,12 @@ def test_a_prompt_among_single_tokens(ctx, t, io, D, at):
     lens = tokens[:at] + [(130, 200)] + tokens[at:]
     for heads, nh, more in ((1, 3, {}), (8, 8, {"spare_rows": 5, "mask": True, "causal": False})):
         Batch(ctx, t, io, heads, nh, D, 64, lens, seed=at + D, **more).check()
+
+
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D", [64, 96])
+def test_a_prompt_beside_a_long_token(ctx, io, D):
+    # many key ranges, joined row by row where the bounds hold far more rows than there are
+    x = Batch(ctx, ref.Q4_0, io, 1, 2, D, 64, [(1, 10), (33, 300), (0, 50), (1, 4000), (1, 0)], seed=D, spare_rows=2)
+    assert s3e.kv_attn_workspace(x.c, x.b, 2, io) > 8 * x.n_tokens * 2 * (D + 2) * 4
+    x.check()

@@ -12,14 +12,14 @@ namespace s3e {
 //   K words | K scales | V words | V scales.
 // A word is eight codes (4 bytes of Q4_0 nibbles, 8 bytes of Q8_0): what one
 // lane feeds to one 16 × 16 × 32 fp16 MFMA as eight consecutive values of the
-// summed dimension, so attention goes from memory to the matrix cores without
-// LDS or shuffles.  K: key r = 8a + 4t + i of the chunk (a, i < 4, t < 2) and
-// channels 32b + 8g + j (j < 8) are word t·NB + b of lane 16g + 4a + i.  V:
-// channel 16w + m and keys 8g + j are word w of lane 16g + m.  Either way a
-// lane has 2·NB words; they lie in pieces of up to 16 bytes a lane, all 64
-// lanes of a piece together, so that a wave's load of a piece is contiguous.
-// Code j of a Q4_0 word is nibble (j >> 1) + 4·(j & 1) (two codes of one shift
-// then sit 16 bits apart, as an fp16 pair needs them), of a Q8_0 word byte j.
+// summed dimension, so attention takes words as they lie, without shuffles.  K:
+// key r = 8a + 4t + i of the chunk (a, i < 4, t < 2) and channels 32b + 8g + j
+// (j < 8) are word t·NB + b of lane 16g + 4a + i.  V: channel 16w + m and keys
+// 8g + j are word w of lane 16g + m.  Either way a lane has 2·NB words; they
+// lie in pieces of up to 16 bytes a lane, all 64 lanes of a piece together, so
+// that a wave's load of a piece is contiguous. Code j of a Q4_0 word is nibble
+// (j >> 1) + 4·(j & 1) (two codes of one shift then sit 16 bits apart, as an
+// fp16 pair needs them), of a Q8_0 word byte j.
 // Scales are fp16 [NB][32 keys].
 template <int Q, int NB>
 struct KvChunk {

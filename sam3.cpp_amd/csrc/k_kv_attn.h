@@ -6,14 +6,15 @@
 // reference and sum.  Both products run transposed on the 16 × 16 × 32 fp16
 // MFMA: Sᵀ = K·Qᵀ, then Oᵀ = Vᵀ·Pᵀ, so that a lane's scores (column lane % 16,
 // keys 8·(lane / 16) .. + 8 of a chunk of 32) are its operand of the second
-// product as they stand, and the words of both tensors (k_kv.h) go from
-// memory to the matrix core through registers alone.
+// product as they stand, and so are the words of both tensors (k_kv.h) once
+// their codes are fp16.
 //
 // Codes are exact in fp16, and a block of 32 channels is the summed dimension
 // of one MFMA, so K's scale multiplies each block sum in fp32: scores carry no
 // rounding but q's own.  V's scale varies along the summed dimension and goes
 // into the probabilities: P·d is rounded once, to fp16 (fp32 operands: kept as
-// a pair hi + lo, as is q, scaled by its row's power of two).  So that P·d
+// a pair hi + lo, as is q, scaled by its row's power of two; over few keys in
+// fp16 too).  So that P·d
 // stays below fp16's largest and well above its smallest, a column's exponents
 // are measured from a reference: its largest score so far plus the exponent of
 // the largest scale of V among the keys it has seen; both are taken again, and

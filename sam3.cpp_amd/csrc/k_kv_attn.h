@@ -149,6 +149,7 @@ typedef __attribute__((address_space(4))) const int32_t c_i32;
 struct KvTask {
     bool some;
     int split, kvh, q0, nq, ncols, len, c0, G;
+    int before;          // under a causal mask row i sees the first before + i + 1 keys, of len (which may end before them)
     int k_begin, k_end;  // of the tile: keys some of its columns see
 };
 template <int COLS>
@@ -200,12 +201,14 @@ __device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
     t.ncols = min(t.nq, a.max_q) * t.G;
     t.c0 = ct * COLS;
     if (t.c0 >= t.ncols) return t;
-    t.len = (int)min((int64_t)max(a.kv_len[s], 0), a.max_kv);
+    const int kv = max(a.kv_len[s], 0);
+    t.len = (int)min((int64_t)kv, a.max_kv);
+    t.before = kv - t.nq;
     const int64_t kb = t.split * a.chunk;
     if (kb >= t.len && t.split > 0) return t;  // past the sequence: no range the joining pass reads
     const int i_last = (min(t.c0 + COLS, t.ncols) - 1) / t.G;
     t.k_begin = (int)kb;
-    t.k_end = (int)min((int64_t)(a.causal ? min(t.len, t.len - t.nq + i_last + 1) : t.len), kb + a.chunk);
+    t.k_end = (int)min((int64_t)(a.causal ? min(t.len, t.before + i_last + 1) : t.len), kb + a.chunk);
     t.some = true;
     return t;
 }
@@ -255,7 +258,7 @@ struct KvColumns {
         const int col = lane & 15, ka = lane >> 4;
         c0 = first;
         const int i_first = min(c0, k.ncols - 1) / k.G;
-        see_all = a.causal ? min(k.len, k.len - k.nq + i_first + 1) : k.len;
+        see_all = a.causal ? min(k.len, k.before + i_first + 1) : k.len;
         bound = 0x7fff;
 #pragma unroll
         for (int n = 0; n < NT; n++) {
@@ -382,7 +385,7 @@ struct KvColumns {
                         t[n][j] = mv[j] == -INFINITY ? -INFINITY : __builtin_fmaf(mv[j], 1.4426950408889634f, t[n][j] * cs[n]);
                 }
                 hidden[n] = 0;
-                const int lim = a.causal ? min(k.len, k.len - k.nq + tok[n] - k.q0 + 1) : k.len;
+                const int lim = a.causal ? min(k.len, k.before + tok[n] - k.q0 + 1) : k.len;
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     if (!have || key0 + j >= lim) t[n][j] = -INFINITY;
@@ -775,7 +778,7 @@ __global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) vo
     cols.start(a, k, k.c0 + wave * 16, lane);
     // this wave's own columns see no key from here on
     const int i_last = (min(cols.c0 + 16, k.ncols) - 1) / k.G;
-    const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.len - k.nq + i_last + 1 : k.len);
+    const int see_any = cols.c0 >= k.ncols ? 0 : min(k.k_end, a.causal ? k.before + i_last + 1 : k.len);
     if (n > 0) {
         convert(smem);
         if (n > 1) {

@@ -638,3 +638,12 @@ def test_a_prompt_beside_a_long_token(ctx, io, D):
     x = Batch(ctx, ref.Q4_0, io, 1, 2, D, 64, [(1, 10), (33, 300), (0, 50), (1, 4000), (1, 0)], seed=D, spare_rows=2)
     assert s3e.kv_attn_workspace(x.c, x.b, 2, io) > 8 * x.n_tokens * 2 * (D + 2) * 4
     x.check()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D,lens", [(64, [(2, 200), (5, 130), (1, 100)]), (128, [(40, 150), (3, 128), (1, 900)]),
+                                    (256, [(150, 200), (150, 140)]), (64, [(1, 300), (1, 20), (70, 190), (1, 129), (1, 131)])])
+def test_causal_rows_of_sequences_longer_than_max_kv(ctx, t, io, D, lens):
+    # row i of nq sees keys up to kv_len - nq + i, cut at max_kv: not up to max_kv - nq + i
+    Batch(ctx, t, io, 1, 2, D, 64, lens, seed=D, max_kv=128).check()

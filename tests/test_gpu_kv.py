@@ -647,3 +647,35 @@ def test_a_prompt_beside_a_long_token(ctx, io, D):
 def test_causal_rows_of_sequences_longer_than_max_kv(ctx, t, io, D, lens):
     # row i of nq sees keys up to kv_len - nq + i, cut at max_kv: not up to max_kv - nq + i
     Batch(ctx, t, io, 1, 2, D, 64, lens, seed=D, max_kv=128).check()
+
+
+def few_keys_bound(o, bound, visible):
+    """A bound for fp16 rows by the keys that they see (their sequence's length and the causal limit): up to 128 of them
+    fp32's, and the output's rounding to fp16 (2^-11, and 2^-25 below its normal numbers)."""
+    few = visible <= 128
+    return few, bound * (1 + 2.0 ** -11) + np.abs(o) * 2.0 ** -11 + 2.0 ** -25
+
+
+def check_few_keys(x, n_checked):
+    got, at, checked = x.run().astype(np.float64), 0, 0
+    for i, (n, keys) in enumerate(x.lens):
+        parts = [p[at:at + keys] for y in (x.k, x.v) for p in ref.quantize(x.t, y)]
+        at += keys
+        see = np.arange(keys) <= (keys - n + np.arange(n)[:, None]) if x.causal else np.ones((n, keys), bool)
+        rows_ = slice(x.starts[i], x.starts[i + 1])
+        q = x.q[rows_, :x.nh * x.D].reshape(n, x.nh, x.D)
+        o, mag, A = ref.attention(x.t, *parts, q, x.scale, see)
+        few, bound = few_keys_bound(o, ref.attention_bound(True, o, mag, A, keys, x.D, ref.largest(x.t, *parts[2:])), see.sum(-1))
+        off = np.abs(got[rows_] - o)
+        assert (off[few] <= bound[few]).all(), (i, (off[few] / bound[few]).max())
+        checked += few.sum()
+    assert checked == n_checked
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nq,kv,causal", [(100, 128, True), (300, 128, False), (300, 40, False)])
+def test_many_columns_of_few_keys_round_once(ctx, t, nq, kv, causal):
+    # head dim 256, more columns than one work-group of the other kernel takes.  (A small scale: the bound of the scores'
+    # own roundings, 2^-24 · (D + 8) · their size, would hide one of P·d at this head dim)
+    x = Batch(ctx, t, s3e.TYPE_F16, 1, 1, 256, 64, [(nq, kv)], seed=nq + kv, causal=causal, scale=1e-4)
+    check_few_keys(x, nq)

@@ -335,8 +335,10 @@ int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t 
  * quantized K and V: query head h reads key/value head h / (nh / n_heads).
  * Q(row, h, d) = q[row·q_nb[0] + h·q_nb[1] + d]; o is [n_tokens][nh][D]
  * (16-byte aligned), of the same `type`:
- *   S3E_TYPE_F16  q in fp16, probabilities times V's scales rounded to fp16
- *                 where max_kv is over 128 (fp32 scores, sums and accumulation);
+ *   S3E_TYPE_F16  q in fp16, probabilities times V's scales as fp16 pairs in
+ *                 rows that see at most 128 keys by kv_len, max_kv and the
+ *                 causal limit (a mask's hidden ones count), elsewhere rounded
+ *                 to fp16 (fp32 scores, sums and accumulation);
  *   S3E_TYPE_F32  q and those products as fp16 pairs: fp32 attention to ~1e-6.
  * causal: row i of a sequence's nq sees keys 0 .. kv_len − nq + i; otherwise
  * all kv_len of them.  mask (NULL: none): fp16, mask[row·mask_ld + key] is
@@ -344,7 +346,9 @@ int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t 
  * key's scales and codes reach no result, whatever they are, nor does a page
  * the cache does not have (its keys are hidden).  A row that sees no key is
  * zero.  Rows outside every sequence are left as they are, and so are rows
- * of a sequence past max_q; keys past max_kv are not seen.  o may be q itself
+ * of a sequence past max_q; keys past max_kv are not seen.  The batch's counts
+ * choose the ranges of keys that are summed apart, so a row's last bits may
+ * differ between batches; how many it holds does not.  o may be q itself
  * (same type, contiguous) but overlaps nothing else that the call reads.
  * ws: device, 16-byte aligned, ws_bytes of it, this call's own until it has
  * run and outside all of the above; with it the call allocates nothing and can

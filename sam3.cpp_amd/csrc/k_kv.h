@@ -83,7 +83,6 @@ struct KvAttnArgs {
     int64_t max_kv = 0;
     int tile = 0;           // the kernel for many columns
     int nt = 1;             // column tiles of 16 a wave
-    int pairs = 0;          // fp16 operands: probabilities as pairs all the same
     int ctiles = 1;         // work-groups over the columns of a sequence and head
     // > 0: work-groups over the columns of all sequences and one head, found by
     // q_start, instead of ctiles for each
@@ -100,8 +99,8 @@ hipError_t launch_kv_attn_q4(const KvAttnArgs &a, bool f32, hipStream_t st);
 hipError_t launch_kv_attn_q8(const KvAttnArgs &a, bool f32, hipStream_t st);
 hipError_t launch_kv_combine(const KvAttnArgs &a, bool f32, hipStream_t st);
 // The kernel, column tiles and work-groups over the columns where a sequence and
-// head have up to `cols` of them, all sequences `all_cols`, against up to `keys` keys.
-void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols, int64_t all_cols, int64_t keys);
+// head have up to `cols` of them, all sequences `all_cols`.
+void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols, int64_t all_cols);
 
 // The reference exponent of a column that has seen no key.
 constexpr float KV_NONE = -3.0e38f;

@@ -14,7 +14,7 @@
 // rounding but q's own.  V's scale varies along the summed dimension and goes
 // into the probabilities: P·d is rounded once, to fp16 (fp32 operands: kept as
 // a pair hi + lo, as is q, scaled by its row's power of two; over few keys in
-// fp16 too).  So that P·d
+// fp16 too, KV_FEW_KEYS).  So that P·d
 // stays below fp16's largest and well above its smallest, a column's exponents
 // are measured from a reference: its largest score so far plus the exponent of
 // the largest scale of V among the keys it has seen; both are taken again, and
@@ -144,10 +144,20 @@ constexpr int vm_wait(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (
 // every chunk under way).
 typedef __attribute__((address_space(4))) const int32_t c_i32;
 
+// Up to so many keys a row's P·d are pairs in fp16 too: the roundings of few hardly
+// average (up to as much again as the output's own).  A work-group decides it by the
+// keys its first row sees, so that no bound of the batch and no other sequence has a
+// part in it.  µs rounded once and as pairs for every row: 64 sequences' tokens over up
+// to 4096 keys (8 heads of 128, Q4_0) 50 and 61, 4 × 2048 queries (16 heads of 64) 109
+// and 148, 4096 × 28 736 at head dim 256 240 and 359; with few keys, where both take the
+// loads' and the launch's time, 64 × 512 × 128 at head dim 256 53 and 61.
+constexpr int KV_FEW_KEYS = 128;
+
 // What a work-group is to do: its sequence, key/value head, key range and
 // first column; `some` where there is anything.
 struct KvTask {
     bool some;
+    bool few;  // of the work-group's rows the first sees at most KV_FEW_KEYS keys (by length and causal limit)
     int split, kvh, q0, nq, ncols, len, c0, G;
     int before;          // under a causal mask row i sees the first before + i + 1 keys, of len (which may end before them)
     int k_begin, k_end;  // of the tile: keys some of its columns see
@@ -206,7 +216,8 @@ __device__ __forceinline__ KvTask kv_task(const KvAttnArgs &a, int &s) {
     t.before = kv - t.nq;
     const int64_t kb = t.split * a.chunk;
     if (kb >= t.len && t.split > 0) return t;  // past the sequence: no range the joining pass reads
-    const int i_last = (min(t.c0 + COLS, t.ncols) - 1) / t.G;
+    const int i_first = t.c0 / t.G, i_last = (min(t.c0 + COLS, t.ncols) - 1) / t.G;
+    t.few = (a.causal ? min(t.len, t.before + i_first + 1) : t.len) <= KV_FEW_KEYS;
     t.k_begin = (int)kb;
     t.k_end = (int)min((int64_t)(a.causal ? min(t.len, t.before + i_last + 1) : t.len), kb + a.chunk);
     t.some = true;
@@ -614,22 +625,19 @@ constexpr int KV_STAGES = 2, KV_WAVES = 4;
 // Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
 // through an accumulation register; more where the registers suffice.
 constexpr int kv_waves(int Q, int NB, int NT) { return NT > 1 || NB == 8 || Q * NB == 32 ? 2 : (NB <= 2 ? 4 : 3); }
+// … of the kernel that holds both forms of fp16's P·d: at head dim 64 the pairs would
+// take it past 128 registers, and prompts 118 µs for 109 (with it they have 6 or 7 in memory).
+constexpr int kv_bound(int Q, int NB, bool F32, int NT) { return !F32 && NT > 1 && NB == 2 ? 4 : kv_waves(Q, NB, NT); }
 
 template <int Q, int NB, bool F32, int NT, bool PAIRS>
-__global__ __launch_bounds__(64 * KV_WAVES, kv_waves(Q, NB, NT)) void k_kv_attn(KvAttnArgs a) {
+__device__ __forceinline__ void kv_rings(const KvAttnArgs &a, const KvTask &k, int s, uint8_t *smem) {
     using C = KvChunk<Q, NB>;
     using Cols = KvColumns<NB, F32, NT, false, PAIRS>;
     constexpr int W = Cols::W, WAVES = KV_WAVES;
     constexpr int LD = (C::BYTES + 1023) / 1024;  // 1 KB loads of a chunk
-    // at the end the accumulators of two waves
-    constexpr int RING = WAVES * KV_STAGES * C::BYTES, JOIN = 2 * NT * (W * 1024 + 512);
-    __shared__ __attribute__((aligned(16))) uint8_t smem[RING > JOIN ? RING : JOIN];
 
     const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int s;
-    const KvTask k = kv_task<16 * NT>(a, s);
-    if (!k.some) return;
     const KvPlaces places(a, s, k.kvh, C::BYTES);
 
     const int g_end = (k.k_end + 31) >> 5;
@@ -706,6 +714,18 @@ __global__ __launch_bounds__(64 * KV_WAVES, kv_waves(Q, NB, NT)) void k_kv_attn(
     cols.store(a, k, lane);
 }
 
+template <int Q, int NB, bool F32, int NT>
+__global__ __launch_bounds__(64 * KV_WAVES, kv_bound(Q, NB, F32, NT)) void k_kv_attn(KvAttnArgs a) {
+    // the rings; at the end the accumulators of two waves
+    constexpr int RING = KV_WAVES * KV_STAGES * KvChunk<Q, NB>::BYTES, JOIN = 2 * NT * (2 * NB * 1024 + 512);
+    __shared__ __attribute__((aligned(16))) uint8_t smem[RING > JOIN ? RING : JOIN];
+    int s;
+    const KvTask k = kv_task<16 * NT>(a, s);
+    if (!k.some) return;
+    if (F32 || k.few) kv_rings<Q, NB, F32, NT, true>(a, k, s, smem);
+    else if constexpr (!F32) kv_rings<Q, NB, F32, NT, false>(a, k, s, smem);
+}
+
 // ---- many columns at head dim 256: bound by vector instructions and LDS -------
 // There a wave's registers hold no second column tile to share a chunk's
 // conversion with, and the first kernel's rings leave a CU one or two
@@ -723,19 +743,19 @@ constexpr int KV_TILE_NB = 8;
 constexpr int kv_tile_waves(bool F32) { return F32 ? 8 : 12; }
 constexpr int kv_tile_cols(bool F32) { return 16 * kv_tile_waves(F32); }
 
-template <int Q, bool F32>
-__global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) void k_kv_attn_tile(KvAttnArgs a) {
+// bytes of a buffer: K, V operands, K, V scales
+template <int Q>
+constexpr int KV_TILE_BUF = 2 * KvChunk<Q, KV_TILE_NB>::WORDS * 1024 + 2 * KvChunk<Q, KV_TILE_NB>::SCALES;
+
+template <int Q, bool F32, bool PAIRS>
+__device__ __forceinline__ void kv_tile(const KvAttnArgs &a, const KvTask &k, int s, uint8_t *smem) {
     constexpr int NB = KV_TILE_NB, WAVES = kv_tile_waves(F32);
     using C = KvChunk<Q, NB>;
-    using Cols = KvColumns<NB, F32, 1, true, F32>;
-    constexpr int HALF = C::WORDS * 1024, BUF = 2 * HALF + 2 * C::SCALES;  // K, V operands, K, V scales
-    __shared__ __attribute__((aligned(16))) uint8_t smem[4 * BUF];
+    using Cols = KvColumns<NB, F32, 1, true, PAIRS>;
+    constexpr int HALF = C::WORDS * 1024, BUF = KV_TILE_BUF<Q>;
 
     const int tid = threadIdx.x, lane = tid & 63, ka = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int s;
-    const KvTask k = kv_task<kv_tile_cols(F32)>(a, s);
-    if (!k.some) return;
     const KvPlaces places(a, s, k.kvh, C::BYTES);
 
     // pieces of K and V this wave converts; the scales are the last wave's (of fewer pieces)
@@ -810,6 +830,16 @@ __global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) vo
     if (cols.c0 < k.ncols) cols.store(a, k, lane);
 }
 
+template <int Q, bool F32>
+__global__ __launch_bounds__(64 * kv_tile_waves(F32), kv_tile_waves(F32) / 4) void k_kv_attn_tile(KvAttnArgs a) {
+    __shared__ __attribute__((aligned(16))) uint8_t smem[4 * KV_TILE_BUF<Q>];
+    int s;
+    const KvTask k = kv_task<kv_tile_cols(F32)>(a, s);
+    if (!k.some) return;
+    if (F32 || k.few) kv_tile<Q, F32, true>(a, k, s, smem);
+    else if constexpr (!F32) kv_tile<Q, F32, false>(a, k, s, smem);
+}
+
 // Column tiles a wave of the first kernel holds where there are more than 16 columns.
 constexpr int kv_most_tiles(int NB) { return NB == 8 ? 1 : 2; }
 
@@ -824,17 +854,11 @@ hipError_t launch_kv_attn(const KvAttnArgs &a, bool f32, hipStream_t st) {
             if constexpr (NB == KV_TILE_NB) hipLaunchKernelGGL((k_kv_attn_tile<Q, f()>), g, dim3(64 * kv_tile_waves(f())), 0, st, a);
             else return hipErrorInvalidValue;
         } else if (a.nt == 1 || a.nt == MOST) {
-            auto rings = [&](auto nt, auto pairs) {
-                hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), nt(), pairs()>), g, dim3(64 * KV_WAVES), 0, st, a);
-            };
-            auto by_pairs = [&](auto nt) {
-                if (f() || a.pairs) rings(nt, std::true_type{});
-                else if constexpr (!f()) rings(nt, std::false_type{});
-            };
-            if (a.nt == 1) by_pairs(std::integral_constant<int, 1>{});
-            else by_pairs(std::integral_constant<int, MOST>{});
+            if (a.nt == 1) hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), 1>), g, dim3(64 * KV_WAVES), 0, st, a);
+            else hipLaunchKernelGGL((k_kv_attn<Q, NB, f(), MOST>), g, dim3(64 * KV_WAVES), 0, st, a);
+        } else {
+            return hipErrorInvalidValue;
         }
-        else return hipErrorInvalidValue;
         return hipGetLastError();
     };
     auto by = [&](auto nb) { return f32 ? go(nb, std::true_type{}) : go(nb, std::false_type{}); };

@@ -14,15 +14,11 @@ hipError_t launch_kv_attn_q4(const KvAttnArgs &a, bool f32, hipStream_t st) { re
 // 583 / 755, 512 1096 / 1031).  At the smaller head dims a wave holds two column
 // tiles and four or three work-groups share a CU: ahead at every count (4 × 2048
 // queries, 16 heads of 64: 109 against 117; 64 × 256 columns of 128: 278 against 379).
-void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols, int64_t all_cols, int64_t keys) {
+void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols, int64_t all_cols) {
     const int NB = D / 32;
     const bool q4 = a.c.type == S3E_TYPE_Q4_0;
     int64_t per;
-    // few keys: the roundings of their P·d to fp16 hardly average (up to as much
-    // again as the output's own); the kernel that makes pairs of fp16 queries' too is
-    // the first one
-    const bool few = !f32 && keys <= 128;
-    a.tile = NB == KV_TILE_NB && cols > (q4 ? 256 : 64) && !few;
+    a.tile = NB == KV_TILE_NB && cols > (q4 ? 256 : 64);
     if (a.tile) {
         a.nt = 1;
         per = kv_tile_cols(f32);
@@ -32,9 +28,6 @@ void kv_attn_columns(KvAttnArgs &a, int D, bool f32, int64_t cols, int64_t all_c
     } else {
         a.nt = cols <= 16 ? 1 : kv_most_tiles(NB);
         per = 16 * a.nt;
-        // (µs without / with, 256 sequences of 8 heads of 128, 32 query heads, Q4_0: 64
-        // keys 16.7 / 18.1, 256 22.4 / 24.8; one sequence 7.6 / 7.4, 7.7 / 8.4)
-        a.pairs = few;
         // as many as run at once; sequences of unlike length fill the CUs better in
         // more, shorter ranges where three or more share a CU (µs by goal, one of
         // 131 072 keys, 8 heads: Q4_0 × 128 512 39.0, 768 39.3, 1536 43.0; Q8_0 × 128

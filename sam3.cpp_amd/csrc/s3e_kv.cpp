@@ -112,7 +112,7 @@ void plan(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t nh, bool f32, Kv
     a.n_seq = (int)b->n_seq;
     a.c.type = c->type;
     const int64_t G = nh / c->n_heads;
-    kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * G, b->n_tokens * G, b->max_kv);
+    kv_attn_columns(a, c->head_dim, f32, std::min(b->max_q, b->n_tokens) * G, b->n_tokens * G);
     const int64_t wgs = c->n_heads * (a.tiles ? a.tiles : b->n_seq * a.ctiles);
     // (to the nearest: 64 sequences of up to 4096 keys, 16 heads of 64, Q8_0, whose
     // 1024 work-groups are two thirds of the goal, take 64 µs in one range, 70 in two)

@@ -679,3 +679,18 @@ def test_many_columns_of_few_keys_round_once(ctx, t, nq, kv, causal):
     # own roundings, 2^-24 · (D + 8) · their size, would hide one of P·d at this head dim)
     x = Batch(ctx, t, s3e.TYPE_F16, 1, 1, 256, 64, [(nq, kv)], seed=nq + kv, causal=causal, scale=1e-4)
     check_few_keys(x, nq)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("D,lens,causal", [
+    (64, [(1, 20), (1, 2000), (1, 128)], True), (128, [(5, 40), (3, 1000), (2, 129)], False), (96, [(30, 100), (30, 30), (7, 700)], True),
+    (32, [(200, 200)], True), (128, [(140, 300)], True), (64, [(150, 180), (150, 150)], True),
+    (256, [(1, 20), (1, 2000)], True), (256, [(300, 300), (40, 60)], True), (256, [(300, 90), (3, 500)], False),
+    (64, [(130, 130), (1, 5), (1, 900), (1, 0), (1, 60)], True)])
+def test_rows_of_few_keys_round_once_in_any_batch(ctx, t, D, lens, causal):
+    # whatever the batch's bounds, and the later rows of a prompt, are: the first rows of a prompt and short sequences
+    # (heads: of one and of three columns a query; more sequences than the bounds need, so that one finds its own)
+    for heads, nh in ((1, 1), (2, 6)):
+        x = Batch(ctx, t, s3e.TYPE_F16, heads, nh, D, 64, lens, seed=D + nh, causal=causal, scale=1e-4, spare_rows=1)
+        check_few_keys(x, sum(int((np.minimum(kv, kv - nq + np.arange(nq) + 1) <= 128).sum()) if causal else nq * (kv <= 128) for nq, kv in lens))
+        assert (x.run()[x.starts[-1]:] == 5).all()

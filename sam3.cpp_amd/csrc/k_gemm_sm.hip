@@ -78,7 +78,10 @@ __device__ __forceinline__ int half_sum(int v) {
 // in registers, to the bit as the separate conversion pass does.  The strips
 // repeat the conversion (a third of a stage's work), but one launch and the
 // round trip through memory go: 7 × 1024 × 1024 Q4_0 21.7 → 19.2 µs a call.
-template <int WK, int MT, int KS, bool XF = false>
+// FUSED: y = act(W·x + bias) + resid.  (Products without it keep a kernel of
+// their own: with both tested in the loop over outputs, M = 64 Q4_0 took fc1
+// 6.8 → 7.1 µs, fc2 8.7 → 8.9.)
+template <int WK, int MT, int KS, bool XF = false, bool FUSED = false>
 __global__ __launch_bounds__(64 * SM_WAVES, 2) void k_gemm_sm(SmArgs p) {
     using C = SmCfg<WK>;
     constexpr int SPW = SM_WAVES / KS;  // strips per work-group
@@ -319,10 +322,11 @@ __global__ __launch_bounds__(64 * SM_WAVES, 2) void k_gemm_sm(SmArgs p) {
                 for (int w = 1; w < KS; w++) v += red[st * KS + w][row][col];
                 v *= kScale;
                 if (G.bias) v += G.bias[gn];
-                const int64_t at = (int64_t)(r0 + row) * G.ldy + gn;
-                if (p.act) v = act_f32(p.act, v);
-                if (p.resid) v += p.resid[at];
-                G.y[at] = v;
+                if constexpr (FUSED) {
+                    v = act_f32(p.act, v);
+                    if (p.resid) v += p.resid[(int64_t)(r0 + row) * G.ldy + gn];
+                }
+                G.y[(int64_t)(r0 + row) * G.ldy + gn] = v;
             }
             return;
         }
@@ -340,25 +344,44 @@ __global__ __launch_bounds__(64 * SM_WAVES, 2) void k_gemm_sm(SmArgs p) {
     }
 }
 
-// Y = act(scale · Σ_k part[k] + bias) + resid over the kg ≤ SM_KG_MAX partial sums of a
-// split small-M product, added in index order (one thread per output; the kg
-// loads are all issued before the first add).
-__global__ __launch_bounds__(256) void k_sm_reduce(const float *__restrict__ part, int kg, int64_t mn, int N,
-                                                  float scale, const float *__restrict__ bias, float *y, int64_t ldy,
-                                                  int act, const float *resid) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= mn) return;
+// scale · Σ_k part[k] + bias over the kg ≤ SM_KG_MAX partial sums of a split
+// small-M product, added in index order (one thread per output i = row·N + col;
+// the kg loads are all issued before the first add).
+__device__ __forceinline__ float sm_sum(const float *__restrict__ part, int kg, int64_t mn, int N, float scale,
+                                        const float *__restrict__ bias, int64_t i, int64_t &row, int &col) {
     float pv[SM_KG_MAX];
 #pragma unroll
     for (int k = 0; k < SM_KG_MAX; k++) pv[k] = k < kg ? part[k * mn + i] : 0.f;
     float v = 0.f;
 #pragma unroll
     for (int k = 0; k < SM_KG_MAX; k++) v += pv[k];  // + 0 past kg leaves v unchanged
-    const int64_t row = i / N;
-    const int col = (int)(i - row * N);
+    row = i / N;
+    col = (int)(i - row * N);
     v *= scale;
     if (bias) v += bias[col];
-    if (act) v = act_f32(act, v);
+    return v;
+}
+
+__global__ __launch_bounds__(256) void k_sm_reduce(const float *__restrict__ part, int kg, int64_t mn, int N,
+                                                  float scale, const float *__restrict__ bias, float *__restrict__ y,
+                                                  int64_t ldy) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= mn) return;
+    int64_t row;
+    int col;
+    const float v = sm_sum(part, kg, mn, N, scale, bias, i, row, col);
+    y[row * ldy + col] = v;
+}
+
+// Y = act(that) + resid (rows of ldy; may be y)
+__global__ __launch_bounds__(256) void k_sm_reduce_act(const float *__restrict__ part, int kg, int64_t mn, int N,
+                                                      float scale, const float *__restrict__ bias, float *y, int64_t ldy,
+                                                      int act, const float *resid) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= mn) return;
+    int64_t row;
+    int col;
+    float v = act_f32(act, sm_sum(part, kg, mn, N, scale, bias, i, row, col));
     if (resid) v += resid[row * ldy + col];
     y[row * ldy + col] = v;
 }
@@ -694,11 +717,16 @@ hipError_t launch_gemm_sm(WKind kind, const SmArgs &a, int wgs, int ks, hipStrea
         return hipErrorInvalidValue;
     if (a.rt != 1 && (a.rt != 2 || a.M <= 32 || a.many || wgs % (2 * a.kg) != 0)) return hipErrorInvalidValue;
     if (a.x32 && (a.many || (a.M > 32 && a.rt != 2) || a.one.K % 32 != 0 || a.one.ldx < a.one.K)) return hipErrorInvalidValue;
+    // an epilogue belongs to whatever adds the last sums up
+    const bool epi = a.act || a.resid, fused = epi && a.kg == 1;
     const dim3 grid((unsigned)wgs), block(64 * SM_WAVES);
     const bool two = a.M > 32 && a.rt == 1;
+    if (epi && (a.many || two)) return hipErrorInvalidValue;
 #define S3E_SM(WK)                                                                                       \
     do {                                                                                                 \
-        if (a.x32) hipLaunchKernelGGL((k_gemm_sm<WK, 1, 4, true>), grid, block, 0, st, a);               \
+        if (a.x32 && fused) hipLaunchKernelGGL((k_gemm_sm<WK, 1, 4, true, true>), grid, block, 0, st, a); \
+        else if (fused) hipLaunchKernelGGL((k_gemm_sm<WK, 1, 4, false, true>), grid, block, 0, st, a);   \
+        else if (a.x32) hipLaunchKernelGGL((k_gemm_sm<WK, 1, 4, true>), grid, block, 0, st, a);          \
         else if (two) hipLaunchKernelGGL((k_gemm_sm<WK, 2, 4>), grid, block, 0, st, a);                  \
         else hipLaunchKernelGGL((k_gemm_sm<WK, 1, 4>), grid, block, 0, st, a);                           \
     } while (0)
@@ -715,8 +743,13 @@ hipError_t launch_gemm_sm(WKind kind, const SmArgs &a, int wgs, int ks, hipStrea
     const SmGemm &g = a.one;
     const int64_t mn = (int64_t)a.M * g.N;
     const float scale = kind == WK_F16 ? 1.0f : 0.5f;  // the quantized scale products are doubled
-    hipLaunchKernelGGL(k_sm_reduce, dim3((unsigned)((mn + 255) / 256)), dim3(256), 0, st, (const float *)a.part, a.kg,
-                       mn, g.N, scale, g.bias, g.y, g.ldy, a.act, a.resid);
+    const dim3 rgrid((unsigned)((mn + 255) / 256));
+    if (epi)
+        hipLaunchKernelGGL(k_sm_reduce_act, rgrid, dim3(256), 0, st, (const float *)a.part, a.kg, mn, g.N, scale, g.bias,
+                           g.y, g.ldy, a.act, a.resid);
+    else
+        hipLaunchKernelGGL(k_sm_reduce, rgrid, dim3(256), 0, st, (const float *)a.part, a.kg, mn, g.N, scale, g.bias, g.y,
+                           g.ldy);
     return hipGetLastError();
 }
 

@@ -272,11 +272,14 @@ _held = {}
 
 
 def _engine():
-    """The engine's binding and one context."""
+    """The engine's binding and one context, whose stream torch works on from then on: what torch makes is there before
+    the engine's calls, and torch's later work on their results, and on memory that their inputs leave, waits for them."""
     if "ctx" not in _held:
         sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "sam3.cpp_amd"))
         import s3e
         _held["s3e"], _held["ctx"] = s3e, s3e.Context(0)
+        torch.cuda.synchronize()
+        torch.cuda.set_stream(torch.cuda.ExternalStream(_held["ctx"].stream))
     return _held["s3e"], _held["ctx"]
 
 
@@ -344,9 +347,10 @@ def _prepare_product(case, seed):
 
 
 def prepare(case, seed):
+    if own:
+        _engine()
     s = {"cache": _prepare_cache, "attn": _prepare_attn, "product": _prepare_product}[case["kind"]](case, seed)
     s["case"] = case
-    # the engine's stream is not torch's: what torch made must be there before the first call
     torch.cuda.synchronize()
     return s
 

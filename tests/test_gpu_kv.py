@@ -694,3 +694,24 @@ def test_rows_of_few_keys_round_once_in_any_batch(ctx, t, D, lens, causal):
         x = Batch(ctx, t, s3e.TYPE_F16, heads, nh, D, 64, lens, seed=D + nh, causal=causal, scale=1e-4, spare_rows=1)
         check_few_keys(x, sum(int((np.minimum(kv, kv - nq + np.arange(nq) + 1) <= 128).sum()) if causal else nq * (kv <= 128) for nq, kv in lens))
         assert (x.run()[x.starts[-1]:] == 5).all()
+
+
+IN_PLACE = [
+    # t, heads, nh, D, lens, causal: one range of keys, so that the attention kernel itself stores over q; several column
+    # tiles of a sequence, rows that see no key, sequences without keys, grouped heads
+    (ref.Q4_0, 1, 1, 64, [(70, 200), (3, 2), (1, 0)], True), (ref.Q8_0, 2, 6, 64, [(70, 100), (33, 33)], False),
+    (ref.Q8_0, 1, 3, 128, [(50, 20), (1, 7)], True), (ref.Q4_0, 2, 4, 32, [(1, 90), (1, 0), (1, 250)], True),
+    # the kernel for many columns at head dim 256: a last work-group with waves that hold no column
+    (ref.Q8_0, 1, 1, 256, [(150, 200)], False), (ref.Q8_0, 1, 2, 256, [(110, 20), (140, 240)], True),
+    (ref.Q4_0, 1, 1, 256, [(300, 200), (5, 0)], True), (ref.Q8_0, 1, 1, 256, [(200, 0), (1, 3)], True)]
+
+
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("t,heads,nh,D,lens,causal", IN_PLACE)
+def test_attention_in_one_range_writes_in_place(ctx, io, t, heads, nh, D, lens, causal):
+    x = Batch(ctx, t, io, heads, nh, D, 64, lens, seed=len(lens) + D, causal=causal)
+    assert s3e.kv_attn_workspace(x.c, x.b, nh, io) == 0
+    apart = x.check()
+    for _ in range(3):
+        x.qd.upload(x.q)
+        assert np.array_equal(x.run(o=x.qd), apart)

@@ -266,7 +266,8 @@ extern "C" int s3e_kv_attn(s3e_ctx *ctx, const s3e_kv_cache *c, const s3e_kv_bat
     a.mask_vec = (uintptr_t)mask % 16 == 0 && mask_ld % 8 == 0;
     a.o = o;
     a.sign = scale < 0 ? -1 : (scale > 0 ? 1 : 0);
-    a.scale = a.sign ? std::max((float)(std::fabs((double)scale) * 1.4426950408889634), 1.17549435e-38f) : 1.0f;
+    // (in log2 units, neither zero nor infinite: a score of 0 stays 0)
+    a.scale = a.sign ? (float)std::min(std::max(std::fabs((double)scale) * 1.4426950408889634, 1.17549435e-38), 3.40282347e38) : 1.0f;
     a.causal = causal != 0;
     a.n_tokens = (int)b->n_tokens;
     a.max_q = (int)std::min(b->max_q, b->n_tokens);

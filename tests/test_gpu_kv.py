@@ -715,3 +715,13 @@ def test_attention_in_one_range_writes_in_place(ctx, io, t, heads, nh, D, lens, 
     for _ in range(3):
         x.qd.upload(x.q)
         assert np.array_equal(x.run(o=x.qd), apart)
+
+
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("scale", [3.4e38, -3.4e38, 1e-45])
+def test_scales_at_the_ends_of_fp32(ctx, io, scale):
+    # queries of zeros: every score is zero, whatever the finite scale, and the output V's mean
+    x = Batch(ctx, ref.Q8_0, io, 1, 2, 64, 64, [(3, 100), (20, 40)], seed=4, scale=scale, causal=False)
+    x.q[:] = 0
+    x.qd.upload(x.q)
+    x.check()

@@ -339,7 +339,10 @@ int s3e_kv_attn_workspace(const s3e_kv_cache *c, const s3e_kv_batch *b, int64_t 
  *                 rows that see at most 128 keys by kv_len, max_kv and the
  *                 causal limit (a mask's hidden ones count), elsewhere rounded
  *                 to fp16 (fp32 scores, sums and accumulation);
- *   S3E_TYPE_F32  q and those products as fp16 pairs: fp32 attention to ~1e-6.
+ *   S3E_TYPE_F32  q and those products as fp16 pairs: fp32 attention to ~1e-6 of
+ *                 sum p·|V|, and to 2^-31 a key of the largest |V| that the row
+ *                 sees: a key or a block of 32 channels whose scale is 2^-13 of
+ *                 the largest keeps ~2e-6, one at 2^-17 ~3e-5.
  * causal: row i of a sequence's nq sees keys 0 .. kv_len − nq + i; otherwise
  * all kv_len of them.  mask (NULL: none): fp16, mask[row·mask_ld + key] is
  * added for every head, mask_ld at least max_kv; −∞ hides the key.  A hidden

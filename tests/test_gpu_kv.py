@@ -725,3 +725,19 @@ def test_scales_at_the_ends_of_fp32(ctx, io, scale):
     x.q[:] = 0
     x.qd.upload(x.q)
     x.check()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("io", [s3e.TYPE_F16, s3e.TYPE_F32])
+@pytest.mark.parametrize("D,nq,kv", [(64, 3, 90), (128, 40, 300), (256, 150, 200)])
+def test_channel_blocks_of_unlike_size(ctx, t, io, D, nq, kv):
+    # V's first 32 channels 2^10 times the others, every other key 2^6 times its neighbour: the bound's 2^-31 of the
+    # largest |V| a key is what small blocks and small keys are held to
+    x = Batch(ctx, t, io, 1, 2, D, 64, [(nq, kv)], seed=D + nq)
+    x.v *= np.float32(2.0 ** -6)
+    x.v[:, :, 32:] *= np.float32(2.0 ** -10)
+    x.v[::2] *= np.float32(2.0 ** 6)
+    table = x.arrays[2].download(np.int32, (1, -(-kv // 64)))
+    slots = np.array([table[0, j // 64] * 64 + j % 64 for j in range(kv)], np.int32)
+    ctx.kv_write(x.c, s3e.TYPE_F32, ctx.to_device(x.k), (D, D), ctx.to_device(x.v), (D, D), ctx.to_device(slots), kv)
+    x.check()

@@ -173,13 +173,14 @@ constexpr int KV_ROWS = 64;  // rows of a work-group, four threads each
 // 64-bit atomic or a byte store, so that runs, lone rows and neighbouring
 // work-groups never write each other's codes.
 // Reads the rows and writes 9/16 (Q4_0) or 17/16 bytes a value once: 65 536
-// tokens of 8 heads of 128, fp16 to Q4_0, take 81 µs (344 MB, 4.3 TB/s; a copy
-// of as many bytes 62), 28 736 of one head of 256 to Q8_0 16 µs.  Vector
+// tokens of 8 heads of 128, fp16 to Q4_0, take 81 µs write after write (344 MB,
+// 4.3 TB/s; a copy of as many bytes 62), 92 in turn with reads of them, 28 736 of
+// one head of 256 to Q8_0 16 µs.  Vector
 // instructions keep 73 % of the SIMDs' cycles busy, the more so as memory waits
 // on them: hence the packed range search, the row prefetched ahead of its slot,
 // and the byte transposes that make V's words.  Scattered rows cost a 64-bit
-// atomic for two words: 32 768 of those tokens 215 µs in Q4_0 (an and and an
-// or a word: 1464), 123 µs in Q8_0; 512 of 16 heads of 64 8 µs.
+// atomic for two words: 32 768 of those tokens 209-215 µs in Q4_0 (an and and an
+// or a word: 1464), 115-123 µs in Q8_0; 512 of 16 heads of 64 8 µs.
 template <int Q, int NB, typename T>
 __global__ __launch_bounds__(256) void k_kv_write(KvWriteArgs a) {
     using C = KvChunk<Q, NB>;
@@ -391,7 +392,7 @@ __device__ __forceinline__ void store8(T *o, const float *v) {
 // own codes are picked out of them; the codes meet in LDS as bytes and leave
 // row by row, so that both sides of memory see whole lines.  A slot outside the
 // cache reads as zeros.  Bound by HBM: 65 536 tokens of 8 heads of 128 from Q4_0
-// to fp16 take 84 µs (344 MB, 4.1 TB/s), 28 736 of one head of 256 from Q8_0
+// to fp16 take 85 µs (344 MB, 4.1 TB/s), 28 736 of one head of 256 from Q8_0
 // 12 µs; a code at a time straight to memory took 154 and 15.
 template <int Q, int NB, typename T>
 __global__ __launch_bounds__(256) void k_kv_read(KvReadArgs a) {

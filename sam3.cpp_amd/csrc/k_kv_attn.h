@@ -20,6 +20,9 @@
 // the largest scale of V among the keys it has seen; both are taken again, and
 // the accumulators scaled, when a score exceeds its by 6 or a scale is over
 // twice to four times the largest (P·d is at most 2^7 then, 2^15 in between).
+// One reference serves every key and block of channels: of a key or block whose
+// scale is 2^-13 of the largest, a pair's low half ends at fp16's 2^-24, 2^-19 of
+// the product.
 #pragma once
 
 #include "k_kv.h"
@@ -613,7 +616,7 @@ struct KvColumns {
 // take chunks in turn and are joined in LDS.  Each wave keeps a ring of two
 // chunks in LDS, loaded straight into it: while one is worked on the next is
 // under way without holding registers, so that two to four work-groups share a
-// CU and no wave waits for another before the end.
+// CU (Q8_0 at head dim 256: one) and no wave waits for another before the end.
 // One token of 64 sequences of up to 4096 keys (8 heads of 128, 32 query heads,
 // Q4_0, 174 MB) takes 51 µs with the joining pass, 3.4 TB/s; one of 131 072 keys
 // (151 MB) 41 µs, 3.7 TB/s.  Vector instructions, half of them the conversion of
@@ -623,7 +626,9 @@ struct KvColumns {
 // and matrix instructions of 32 keys and 32 columns take to issue.
 constexpr int KV_STAGES = 2, KV_WAVES = 4;
 // Waves a SIMD is to hold: at least two, so that no MFMA result takes the way
-// through an accumulation register; more where the registers suffice.
+// through an accumulation register; more where the registers suffice.  (The rings
+// of Q8_0 at head dim 256, 139 KB, leave room for one all the same, and 68 to 72
+// accumulation registers are used there.)
 constexpr int kv_waves(int Q, int NB, int NT) { return NT > 1 || NB == 8 || Q * NB == 32 ? 2 : (NB <= 2 ? 4 : 3); }
 // … of the kernel that holds both forms of fp16's P·d: at head dim 64 the pairs would
 // take it past 128 registers, and prompts 118 µs for 109 (with it they have 6 or 7 in memory).

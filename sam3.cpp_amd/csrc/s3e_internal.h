@@ -165,7 +165,7 @@ enum Epi : int {
                      // (hi, lo); with qpool, Q as f32 rows into y for the pooling pass
     EPI_FUSED = 8,   // y = act(acc + bias) + resid          (s3e_mul_mat_act): activation and residual
                      // while the sums are in registers, instead of 98 MB read and written again for
-                     // each (5184 × 4736 × 1024 Q8_0 with its 8 µs conversion: 88-98 µs, with any of them)
+                     // each (5184 × 4736 × 1024 Q8_0 with its 8 µs conversion and GELU: 96-102 µs)
 };
 
 struct EpiArgs {

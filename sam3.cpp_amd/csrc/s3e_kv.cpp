@@ -101,9 +101,9 @@ int check_batch(const char *fn, const s3e_kv_cache *c, const s3e_kv_batch *b, in
     return S3E_OK;
 }
 
-// Fewest keys a work-group is worth starting for (µs at 128, 256, 512, 1024:
-// 7 × 5 queries over up to 1733 keys 19.3, 18.4, 21.3, 26.9; one over 4096 of 16
-// heads of 64 11.2, 10.0, 11.1, 13.3).
+// Fewest keys a work-group is worth starting for (µs at 128, 256, 512, 1024: one
+// query over 4096 keys of 16 heads of 64 10.0, 9.6, 11.2, 13.3; 7 × 5 in fp32
+// under a mask over up to 1733 19.7, 21.3, 26.3, 37.0).
 constexpr int64_t KV_MIN_KEYS = 256;
 
 // The kernel, its column tiles and the split over keys: by the host's bounds

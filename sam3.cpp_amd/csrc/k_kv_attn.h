@@ -149,8 +149,8 @@ typedef __attribute__((address_space(4))) const int32_t c_i32;
 
 // Up to so many keys a row's P·d are pairs in fp16 too: the roundings of few hardly
 // average (up to as much again as the output's own).  A work-group decides it by the
-// keys its first row sees, so that no bound of the batch and no other sequence has a
-// part in it.  µs rounded once and as pairs for every row: 64 sequences' tokens over up
+// keys its first row sees, so that neither the batch's bounds nor other sequences nor
+// a prompt's later rows cost such a row its pairs.  µs rounded once and as pairs for every row: 64 sequences' tokens over up
 // to 4096 keys (8 heads of 128, Q4_0) 50 and 61, 4 × 2048 queries (16 heads of 64) 109
 // and 148, 4096 × 28 736 at head dim 256 240 and 359; with few keys, where both take the
 // loads' and the launch's time, 64 × 512 × 128 at head dim 256 53 and 61.
@@ -630,8 +630,9 @@ constexpr int KV_STAGES = 2, KV_WAVES = 4;
 // of Q8_0 at head dim 256, 139 KB, leave room for one all the same, and 68 to 72
 // accumulation registers are used there.)
 constexpr int kv_waves(int Q, int NB, int NT) { return NT > 1 || NB == 8 || Q * NB == 32 ? 2 : (NB <= 2 ? 4 : 3); }
-// … of the kernel that holds both forms of fp16's P·d: at head dim 64 the pairs would
-// take it past 128 registers, and prompts 118 µs for 109 (with it they have 6 or 7 in memory).
+// The waves a SIMD that k_kv_attn, which holds both forms of fp16's P·d, is compiled
+// for: the pairs' form would take two column tiles at head dim 64 past 128 registers
+// and the prompts from 109 to 118 µs; it has 6 or 7 of them in memory instead.
 constexpr int kv_bound(int Q, int NB, bool F32, int NT) { return !F32 && NT > 1 && NB == 2 ? 4 : kv_waves(Q, NB, NT); }
 
 template <int Q, int NB, bool F32, int NT, bool PAIRS>
